@@ -30,6 +30,10 @@ typedef void* hipStream_t;
 #define TATT_X_BF16 8
 #define TATT_DY_BF16 16
 
+/* element types of the token operators below (tatt_layernorm_*, tatt_rotary, tatt_mha_*) */
+#define TATT_T_F32 0
+#define TATT_T_BF16 1
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -357,6 +361,40 @@ int tatt_image_loss_fwd_bwd(const float* sr, const float* hr, float* per, float 
 
 /* ---- clip_grad_norm_ + Adam over a flat parameter buffer (interfaces/super_resolution_eng.py:277-279) ------ */
 int tatt_clip_adam(float* p, const float* g, float* m, float* v, long n, float lr, float b1, float b2, float eps, float max_norm, float* state, float* workspace, hipStream_t stream);
+
+/* ---- token operators: one transformer layer over image or text tokens of any size -------------------------------------------
+ * The interpreter's own layers (tatt_ln_*, tatt_attn_*, tatt_dec_*) are built for 64 channels, 4 heads x 16 and 26 keys; these take any
+ * width, lengths and head counts, fp32 or bf16 tensors (`dtype` = TATT_T_F32 / TATT_T_BF16; parameters, statistics and sums fp32).
+ * void* tensors are of that type; strides count elements; `strides` arguments are HOST arrays, read during the call.  Tensors may
+ * have any element alignment; 16-byte aligned pointers and strides take the wide loads.  No atomics: results are bit-reproducible.
+ *
+ * LayerNorm over C columns (nn.LayerNorm at model/transformer_v2.py:478-482, :827-831, of any width), optionally with the residual sum in front:
+ *   s = x + res (stored to sum, contiguous, rounded to the type; res = NULL: s = x), y = (s - mu) rstd gamma + beta (NULL: 1 / 0),
+ *   stat[row] = (mu, rstd) for the backward call (may be NULL).  ld* = elements between rows; y, sum, dx contiguous.
+ * tatt_layernorm_bwd: dx = d loss / d s (+ dsum, the gradient that reaches s by other ways; NULL: none), dgamma, dbeta written (each
+ *   may be NULL); workspace tatt_layernorm_workspace floats (NULL if neither is asked for). */
+int tatt_layernorm_fwd(const void* x, long ldx, const void* res, long ldr, const float* gamma, const float* beta, void* sum, void* y, float* stat, long rows, int C, float eps, int dtype, hipStream_t stream);
+size_t tatt_layernorm_workspace(long rows, int C);
+int tatt_layernorm_bwd(const void* s, long lds, const void* dy, long lddy, const void* dsum, long ldds, const float* gamma, const float* stat, void* dx, float* dgamma, float* dbeta, long rows, int C, int dtype, float* workspace, hipStream_t stream);
+
+/* Rotary positions over up to four axes: the first sections[0] dimensions of a head turn by the token's place on axis 0, the next
+ * sections[1] by that on axis 1, ...; dimensions behind the last section pass through.  Pair i of axis a turns by
+ * pos[token][a] * freqs[pair] (device array of sum(sections) / 2 doubles, radians per position); a pair is (i, i + section/2) within
+ * its section, or (2i, 2i + 1) if `interleaved`.  inverse = 1 turns back: the backward pass.  q [B][L][Hq][D], and k with Hk heads in the same
+ * launch (NULL: none), strides (batch, token, head) as HOST arrays of 3; outputs contiguous.  pos: pos_type 0 int64, 1 int32, 2 fp32, strides (batch,
+ * token, axis), 0 where broadcast. */
+int tatt_rotary(const void* q, const long* q_strides, void* q_out, int Hq, const void* k, const long* k_strides, void* k_out, int Hk, const void* pos, int pos_type, const long* pos_strides, const double* freqs, const int* sections, int naxes, int B, long L, int D, int interleaved, int inverse, int dtype, hipStream_t stream);
+
+/* Attention (nn.MultiheadAttention's core at model/transformer_v2.py:476, :819, of any size): q [B][Lq][H][D], k / v [B][Lk][Hkv][D], D <= 128, H a
+ * multiple of Hkv (query head h reads key head h / (H / Hkv)); strides = HOST array of (batch, token, head) for q, k, v (9 values; the
+ * backward call: and out, dout, 15 values).  key_mask (may be NULL): bytes [B][Lk], not 0 = leave the key out, mask_strides (batch, key).  causal: query i
+ * sees key j iff j <= i + Lk - Lq.  out contiguous [B][Lq][H][D]; lse [B][H][Lq] (NULL if no backward call follows).  A row that sees no
+ * key gives zeros, lse = +inf, and no gradient.  The backward call recomputes the probabilities from lse; dq, dk, dv contiguous.
+ * workspace: tatt_mha_*_workspace floats (0 = may be NULL). */
+size_t tatt_mha_fwd_workspace(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype);
+int tatt_mha_fwd(const void* q, const void* k, const void* v, const long* strides, const unsigned char* key_mask, const long* mask_strides, void* out, float* lse, int B, int Lq, int Lk, int H, int Hkv, int D, float scale, int causal, int dtype, float* workspace, hipStream_t stream);
+size_t tatt_mha_bwd_workspace(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype);
+int tatt_mha_bwd(const void* q, const void* k, const void* v, const long* strides, const unsigned char* key_mask, const long* mask_strides, const void* out, const void* dout, const float* lse, void* dq, void* dk, void* dv, int B, int Lq, int Lk, int H, int Hkv, int D, float scale, int causal, int dtype, float* workspace, hipStream_t stream);
 
 #ifdef __cplusplus
 }

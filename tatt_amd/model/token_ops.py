@@ -1,0 +1,271 @@
+"""Operators of a transformer layer over image or text tokens, on the HIP kernels: `layer_norm` (any width, with the residual sum in
+front), `rotary` (positions over several axes: height and width of a map, time of a clip) and `attention` (any lengths, head counts and
+masks).  The interpreter's own layers (transformer_v2.py) run on kernels built for 64 channels, 4 heads x 16 and 26 keys; these are for layers
+of any other size, in fp32 or bf16 (parameters, statistics and sums are fp32).
+
+`layer_norm`, `rotary` and `attention` take part in autograd.  The pairs `*_forward` / `*_backward` are the same launches without it, as the
+engine issues them: explicit outputs, capturable into a hipGraph.  (A `loss.backward()` inside a capture adds to leaves through nodes that an
+earlier eager graph of the same leaves may still hold on another stream; take gradients there with the pairs, or with
+torch.autograd.grad on leaves of the captured program's own.)  Everything runs on the current stream of the tensors' device; results are
+bit-reproducible."""
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ..lib import lib
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+_POS_TYPES = {torch.int64: 0, torch.int32: 1, torch.float32: 2}
+_L2, _L3, _L9, _L15 = (ctypes.c_long * n for n in (2, 3, 9, 15))
+
+
+def _check(what, *tensors):
+    """The tensors' common element type (as the C ABI's number); raises for what the kernels do not take."""
+    t0 = tensors[0]
+    for t in tensors:
+        if not t.is_cuda:
+            raise RuntimeError(f"tatt_amd {what} runs on the GPU only (no CPU fallback)")
+        if t.dtype != t0.dtype or t.device != t0.device:
+            raise RuntimeError(f"tatt_amd {what}: tensors of one type on one device expected, got {t0.dtype} on {t0.device} and {t.dtype} on {t.device}")
+    if t0.dtype not in _DTYPES:
+        raise NotImplementedError(f"tatt_amd {what}: float32 or bfloat16 tensors, got {t0.dtype}")
+    return _DTYPES[t0.dtype]
+
+
+def _call(t, name, *args):
+    """The C entry point on the current stream of t's device."""
+    fn = getattr(lib(), name)
+    if t.device.index != torch.cuda.current_device():
+        with torch.cuda.device(t.device):
+            return fn(*args)
+    return fn(*args)
+
+
+def _rows(t):
+    """t with a contiguous last dimension (a copy only if it has none)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+# ---- layer norm -------------------------------------------------------------------------------------------------------------------
+def _matrix(t):
+    """(t as rows, elements between rows): any leading dimensions that one stride covers, else a contiguous copy."""
+    C = t.shape[-1]
+    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= C:
+        return t, t.stride(0)
+    return t.contiguous(), C
+
+
+def _parameters(what, x, weight, bias):
+    for n, p in (("weight", weight), ("bias", bias)):
+        if p is not None and (p.shape != x.shape[-1:] or p.dtype != torch.float32 or p.device != x.device or not p.is_contiguous()):
+            raise RuntimeError(f"tatt_amd {what}: {n} is a contiguous float32 vector of the last dimension on the input's device, got {tuple(p.shape)} {p.dtype} on {p.device}")
+
+
+def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None, need_stat=True):
+    """-> (y, sum, stat): y = LayerNorm(sum) over the last dimension, sum = x + residual in x's type (x itself without a residual), stat
+    [rows, 2] fp32 = (mean, 1/sqrt(var + eps)) for layer_norm_backward (None unless need_stat)."""
+    dtype = _check("layer_norm", x, *(() if residual is None else (residual,)))
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise RuntimeError("tatt_amd layer_norm: the last dimension is empty")
+    if residual is not None and residual.shape != x.shape:
+        raise RuntimeError(f"tatt_amd layer_norm: the residual has the shape of x, got {tuple(residual.shape)} and {tuple(x.shape)}")
+    _parameters("layer_norm", x, weight, bias)
+    C = x.shape[-1]
+    R = x.numel() // C
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    s = torch.empty_like(y) if residual is not None else x
+    stat = torch.empty(R, 2, dtype=torch.float32, device=x.device) if need_stat else None
+    if R:
+        xm, ldx = _matrix(x)
+        rm, ldr = (None, 0) if residual is None else _matrix(residual)
+        _call(x, "layernorm_fwd", xm, ldx, rm, ldr, weight, bias, None if residual is None else s, y, stat, R, C, eps, dtype)
+    return y, s, stat
+
+
+def layer_norm_backward(dy, s, weight, stat, dsum=None, need_params=True):
+    """-> (ds, dweight, dbias) of layer_norm_forward: ds = the gradient of the sum (x's and the residual's alike), with dsum, what reaches the
+    sum by other ways, added; dweight and dbias fp32 (None unless need_params)."""
+    dtype = _check("layer_norm", s, dy, *(() if dsum is None else (dsum,)))
+    _parameters("layer_norm", s, weight, None)
+    C = s.shape[-1]
+    R = s.numel() // C
+    if dy.shape != s.shape or (dsum is not None and dsum.shape != s.shape) or stat.shape != (R, 2) or stat.dtype != torch.float32 or not stat.is_contiguous():
+        raise RuntimeError("tatt_amd layer_norm_backward: dy and dsum have the shape of the sum, stat is layer_norm_forward's")
+    ds = torch.empty(s.shape, dtype=s.dtype, device=s.device)
+    dw, db = (torch.empty(2, C, dtype=torch.float32, device=s.device) if R else torch.zeros(2, C, device=s.device)).unbind() if need_params else (None, None)
+    if R:
+        sm, lds = _matrix(s)
+        dym, lddy = _matrix(dy)
+        dm, ldd = (None, 0) if dsum is None else _matrix(dsum)
+        ws = torch.empty(lib().layernorm_workspace(R, C), dtype=torch.float32, device=s.device) if need_params else None
+        _call(s, "layernorm_bwd", sm, lds, dym, lddy, dm, ldd, weight, stat, ds, dw, db, R, C, dtype, ws)
+    return ds, dw, db
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps):
+        ctx.set_materialize_grads(False)
+        y, s, stat = layer_norm_forward(x, weight, bias, eps, residual)
+        ctx.save_for_backward(s, weight, stat)
+        return y if residual is None else (y, s)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dsum=None):
+        s, weight, stat = ctx.saved_tensors
+        _, need_r, need_w, need_b, _ = ctx.needs_input_grad
+        if dy is None:                                     # only the sum was used
+            return dsum, dsum if need_r else None, None, None, None
+        ds, dw, db = layer_norm_backward(dy, s, weight, stat, dsum, need_w or need_b)
+        return ds, ds if need_r else None, dw if need_w else None, db if need_b else None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
+    """LayerNorm over the last dimension of x (float32 or bfloat16; weight and bias float32 or None), any width.  With a residual:
+    -> (LayerNorm(sum), sum), sum = x + residual rounded to x's type, in one pass."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight, bias)):
+        return _LayerNormFn.apply(x, residual, weight, bias, eps)
+    y, s, _ = layer_norm_forward(x, weight, bias, eps, residual, need_stat=False)
+    return y if residual is None else (y, s)
+
+
+# ---- rotary positions -------------------------------------------------------------------------------------------------------------
+def rotary_frequencies(sections, base=10000.0, device="cuda"):
+    """Radians per position of every pair, float64 [sum(sections) / 2]: base ** (-2 i / section) for pair i of its section."""
+    return torch.cat([base ** (-torch.arange(0, n, 2, dtype=torch.float64) / n) for n in sections]).to(device)
+
+
+def rotate(q, k, positions, freqs, sections, interleaved=False, inverse=False):
+    """`rotary` without autograd; inverse=True turns back (its backward pass)."""
+    dtype = _check("rotary", q, *(() if k is None else (k,)))
+    n = len(sections)
+    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
+        raise RuntimeError("tatt_amd rotary: q [B, L, H, D] and k [B, L, Hk, D] expected")
+    B, L, H, D = q.shape
+    if not 1 <= n <= 4 or any(s <= 0 or s % 2 for s in sections) or sum(sections) > D:
+        raise RuntimeError(f"tatt_amd rotary: one to four positive even sections of at most {D} dimensions together, got {tuple(sections)}")
+    if positions.dtype not in _POS_TYPES:
+        raise NotImplementedError(f"tatt_amd rotary: positions are int64, int32 or float32, got {positions.dtype}")
+    if positions.device != q.device or tuple(positions.shape) not in ((L, n), (B, L, n), (1, L, n)):
+        raise RuntimeError(f"tatt_amd rotary: positions [L, axes] or [B, L, axes] on the tensors' device expected, got {tuple(positions.shape)} on {positions.device}")
+    if freqs.dtype != torch.float64 or freqs.shape != (sum(sections) // 2,) or freqs.device != q.device or not freqs.is_contiguous():
+        raise RuntimeError("tatt_amd rotary: freqs is a contiguous float64 vector of sum(sections) / 2 on the tensors' device (rotary_frequencies)")
+    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    if qo.numel():
+        q, k = _rows(q), None if k is None or not k.numel() else _rows(k)
+        sp = positions.stride()
+        pos_strides = _L3(sp[0] if len(sp) == 3 and positions.shape[0] > 1 else 0, sp[-2], sp[-1])
+        _call(q, "rotary", q, _L3(*q.stride()[:3]), qo, H, k, None if k is None else _L3(*k.stride()[:3]), ko, 0 if k is None else k.shape[2],
+              positions, _POS_TYPES[positions.dtype], pos_strides, freqs, (ctypes.c_int * n)(*sections), n, B, L, D, bool(interleaved), bool(inverse), dtype)
+    return qo, ko
+
+
+class _RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, freqs, sections, interleaved):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions, freqs)
+        ctx.how = (sections, interleaved)
+        qo, ko = rotate(q, k, positions, freqs, sections, interleaved)
+        return qo if k is None else (qo, ko)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk=None):
+        positions, freqs = ctx.saved_tensors
+        if dq is None and dk is None:
+            return (None,) * 6
+        a, b = (dq, dk) if dq is not None else (dk, None)
+        a, b = rotate(a, b, positions, freqs, *ctx.how, inverse=True)
+        return (a, b, None, None, None, None) if dq is not None else (None, a, None, None, None, None)
+
+
+def rotary(q, k, positions, freqs, sections, interleaved=False):
+    """Rotary positions over several axes.  q [B, L, H, D] and k [B, L, Hk, D] or None (float32 or bfloat16, any strides); positions
+    [L, axes] or [B, L, axes], int64, int32 or float32; the first sections[0] dimensions of each head turn by positions[..., 0], the next
+    sections[1] by positions[..., 1] and so on, the rest passes through; freqs = rotary_frequencies(sections).  -> (q', k'), or q' if k is None."""
+    sections = tuple(int(s) for s in sections)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _RotaryFn.apply(q, k, positions, freqs, sections, bool(interleaved))
+    qo, ko = rotate(q, k, positions, freqs, sections, interleaved)
+    return qo if k is None else (qo, ko)
+
+
+# ---- attention --------------------------------------------------------------------------------------------------------------------
+def _attention_args(q, k, v, mask, scale):
+    dtype = _check("attention", q, k, v)
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise RuntimeError(f"tatt_amd attention: q [B, Lq, H, D] and k, v [B, Lk, Hk, D] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    B, Lq, H, D = q.shape
+    Lk, Hk = k.shape[1:3]
+    if not 0 < D <= 128:
+        raise NotImplementedError(f"tatt_amd attention: heads of 1 to 128 dimensions, got {D}")
+    if Hk == 0 or H == 0 or H % Hk:
+        raise RuntimeError(f"tatt_amd attention: {H} query heads are no multiple of {Hk} key heads")
+    if mask is not None and (mask.dtype != torch.bool or mask.shape != (B, Lk) or mask.device != q.device):
+        raise RuntimeError(f"tatt_amd attention: key_padding_mask is a bool tensor [{B}, {Lk}] on q's device (True = leave the key out), got {tuple(mask.shape)} {mask.dtype} on {mask.device}")
+    return dtype, (B, Lq, Lk, H, Hk, D), D ** -0.5 if scale is None else float(scale)
+
+
+def attention_forward(q, k, v, key_padding_mask=None, causal=False, scale=None, need_lse=True):
+    """-> (out, lse): `attention` without autograd; lse [B, H, Lq] fp32 (None unless need_lse) is what attention_backward recomputes from."""
+    dtype, dims, scale = _attention_args(q, k, v, key_padding_mask, scale)
+    B, Lq, Lk, H, _, D = dims
+    if B == 0 or Lq == 0 or Lk == 0:
+        return q.new_zeros(q.shape), q.new_full((B, H, Lq), float("inf"), dtype=torch.float32) if need_lse else None
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    out = torch.empty(B, Lq, H, D, dtype=q.dtype, device=q.device)
+    lse = torch.empty(B, H, Lq, dtype=torch.float32, device=q.device) if need_lse else None
+    n = lib().mha_fwd_workspace(*dims, dtype)
+    ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
+    mask_strides = None if key_padding_mask is None else _L2(*key_padding_mask.stride())
+    _call(q, "mha_fwd", q, k, v, _L9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]), key_padding_mask, mask_strides, out, lse, *dims,
+          scale, bool(causal), dtype, ws)
+    return out, lse
+
+
+def attention_backward(dout, q, k, v, out, lse, key_padding_mask=None, causal=False, scale=None):
+    """-> (dq, dk, dv) of attention_forward with the same arguments: the probabilities are recomputed from lse."""
+    dtype, dims, scale = _attention_args(q, k, v, key_padding_mask, scale)
+    _check("attention", q, out, dout)
+    B, Lq, Lk, H, Hk, D = dims
+    if out.shape != q.shape or dout.shape != q.shape or lse.shape != (B, H, Lq) or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise RuntimeError("tatt_amd attention_backward: out and dout have the shape of q, lse is attention_forward's")
+    if B == 0 or Lq == 0 or Lk == 0:
+        return q.new_zeros(q.shape), k.new_zeros(k.shape), v.new_zeros(v.shape)
+    q, k, v, out, dout = _rows(q), _rows(k), _rows(v), _rows(out), _rows(dout)
+    dq = torch.empty(B, Lq, H, D, dtype=q.dtype, device=q.device)
+    dk, dv = (torch.empty(B, Lk, Hk, D, dtype=q.dtype, device=q.device) for _ in range(2))
+    ws = torch.empty(lib().mha_bwd_workspace(*dims, dtype), dtype=torch.float32, device=q.device)
+    mask_strides = None if key_padding_mask is None else _L2(*key_padding_mask.stride())
+    _call(q, "mha_bwd", q, k, v, _L15(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *dout.stride()[:3]),
+          key_padding_mask, mask_strides, out, dout, lse, dq, dk, dv, *dims, scale, bool(causal), dtype, ws)
+    return dq, dk, dv
+
+
+class _AttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, mask, causal, scale):
+        out, lse = attention_forward(q, k, v, mask, causal, scale)
+        ctx.save_for_backward(q, k, v, out, lse, mask)
+        ctx.how = (causal, scale)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, mask = ctx.saved_tensors
+        return (*attention_backward(dout, q, k, v, out, lse, mask, *ctx.how), None, None, None)
+
+
+def attention(q, k, v, key_padding_mask=None, causal=False, scale=None):
+    """softmax(scale q k^T) v per head, the scores never in memory.  q [B, Lq, H, D], k and v [B, Lk, Hk, D] (float32 or bfloat16, any
+    strides, D <= 128), H a multiple of Hk: query head h reads key head h // (H // Hk).  key_padding_mask [B, Lk] bool, True = leave the key out (as
+    nn.MultiheadAttention's): nothing of such a key reaches a result.  causal: query i sees keys j <= i + Lk - Lq.  scale: D ** -0.5 if None.  A row
+    that sees no key gives zeros.  -> out [B, Lq, H, D]."""
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _AttentionFn.apply(q, k, v, key_padding_mask, causal, scale)
+    return attention_forward(q, k, v, key_padding_mask, causal, scale, need_lse=False)[0]
