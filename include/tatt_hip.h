@@ -388,8 +388,8 @@ int tatt_rotary(const void* q, const long* q_strides, void* q_out, int Hq, const
 /* Attention (nn.MultiheadAttention's core at model/transformer_v2.py:476, :819, of any size): q [B][Lq][H][D], k / v [B][Lk][Hkv][D], D <= 128, H a
  * multiple of Hkv (query head h reads key head h / (H / Hkv)); strides = HOST array of (batch, token, head) for q, k, v (9 values; the
  * backward call: and out, dout, 15 values).  key_mask (may be NULL): bytes [B][Lk], not 0 = leave the key out, mask_strides (batch, key).  causal: query i
- * sees key j iff j <= i + Lk - Lq.  out contiguous [B][Lq][H][D]; lse [B][H][Lq] (NULL if no backward call follows).  A row that sees no
- * key gives zeros, lse = +inf, and no gradient.  The backward call recomputes the probabilities from lse; dq, dk, dv contiguous.
+ * sees key j iff j <= i + Lk - Lq.  out contiguous [B][Lq][H][D]; lse [B][H][Lq] = base-2 logarithm of the sum of the
+ * exponentials (NULL if no backward call follows).  A row that sees no key gives zeros, lse = +inf, and no gradient.  The backward call recomputes the probabilities from lse; dq, dk, dv contiguous.
  * workspace: tatt_mha_*_workspace floats (0 = may be NULL). */
 size_t tatt_mha_fwd_workspace(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype);
 int tatt_mha_fwd(const void* q, const void* k, const void* v, const long* strides, const unsigned char* key_mask, const long* mask_strides, void* out, float* lse, int B, int Lq, int Lk, int H, int Hkv, int D, float scale, int causal, int dtype, float* workspace, hipStream_t stream);

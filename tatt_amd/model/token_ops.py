@@ -211,7 +211,8 @@ def _attention_args(q, k, v, mask, scale):
 
 
 def attention_forward(q, k, v, key_padding_mask=None, causal=False, scale=None, need_lse=True):
-    """-> (out, lse): `attention` without autograd; lse [B, H, Lq] fp32 (None unless need_lse) is what attention_backward recomputes from."""
+    """-> (out, lse): `attention` without autograd; lse [B, H, Lq] fp32 (None unless need_lse), the base-2
+    logarithm of each row's sum of exponentials (+inf where it sees nothing), is what attention_backward recomputes from."""
     dtype, dims, scale = _attention_args(q, k, v, key_padding_mask, scale)
     B, Lq, Lk, H, _, D = dims
     if B == 0 or Lq == 0 or Lk == 0:

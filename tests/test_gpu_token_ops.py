@@ -22,12 +22,12 @@ def rnd(*shape, seed=0, dtype=F32, scale=1.0):
     return (torch.randn(*shape, generator=g) * scale).to(dtype).cuda()
 
 
-def within(got, ref, terms, dtype, what):
-    """|got - ref| <= STORED |ref| + TERMS terms, everywhere."""
+def within(got, ref, terms, dtype, what, more=0.0):
+    """|got - ref| <= STORED |ref| + (TERMS + more) terms, everywhere."""
     got, ref, terms = got.detach().double().cpu(), ref.detach().cpu(), terms.detach().cpu()
     assert got.shape == ref.shape, what
     assert torch.isfinite(got).all(), f"{what}: not finite"
-    over = (got - ref).abs() - (STORED[dtype] * ref.abs() + TERMS[dtype] * terms + 1e-30)
+    over = (got - ref).abs() - (STORED[dtype] * ref.abs() + (TERMS[dtype] + more) * terms + 1e-30)
     assert over.max() <= 0 if over.numel() else True, f"{what}: over its bound by {float(over.max()):.3e} at {int(over.argmax())} (value {float(ref.flatten()[over.argmax()]):.3e})"
 
 
@@ -99,11 +99,14 @@ def check_attention(q, k, v, do, mask, causal, scale, what):
     assert torch.equal(alone, out)
     with torch.no_grad():
         assert torch.equal(T.attention(q, k, v, mask, causal, scale), out)
+    # the backward pass takes P from the stored lse: rounded once to fp32, it is off by at most half a step = 2^-24 of itself (in units
+    # of the score), and P = exp(S - lse) by that factor: at scores of a thousand 6e-5, more than the rest of the bound
+    seen = torch.isfinite(ref["lse"])
+    stored_lse = 2.0 ** -24 * float(ref["lse"][seen].abs().max()) if seen.any() else 0.0
     for name, got in zip(("out", "dq", "dk", "dv"), (out, *grads)):
-        within(got, *ref[name], dtype, f"{what} {name}")
-    lse, want = lse.cpu().double(), ref["lse"]
+        within(got, *ref[name], dtype, f"{what} {name}", 0.0 if name == "out" else stored_lse)
+    lse, want = lse.cpu().double() * math.log(2.0), ref["lse"]
     assert torch.equal(torch.isinf(lse), torch.isinf(want)), f"{what}: empty rows"
-    seen = torch.isfinite(want)
     assert (lse - want)[seen].abs().max() <= 2.0 ** -15 * max(1.0, float(want[seen].abs().max())) if seen.any() else True, f"{what} lse"
 
 
