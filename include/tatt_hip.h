@@ -374,7 +374,7 @@ int tatt_clip_adam(float* p, const float* g, float* m, float* v, long n, float l
  * tatt_layernorm_bwd: dx = d loss / d s (+ dsum, the gradient that reaches s by other ways; NULL: none), dgamma, dbeta written (each
  *   may be NULL); workspace tatt_layernorm_workspace floats (NULL if neither is asked for). */
 int tatt_layernorm_fwd(const void* x, long ldx, const void* res, long ldr, const float* gamma, const float* beta, void* sum, void* y, float* stat, long rows, int C, float eps, int dtype, hipStream_t stream);
-size_t tatt_layernorm_workspace(long rows, int C);
+size_t tatt_layernorm_workspace(long rows, int C, int dtype);
 int tatt_layernorm_bwd(const void* s, long lds, const void* dy, long lddy, const void* dsum, long ldds, const float* gamma, const float* stat, void* dx, float* dgamma, float* dbeta, long rows, int C, int dtype, float* workspace, hipStream_t stream);
 
 /* Rotary positions over up to four axes: the first sections[0] dimensions of a head turn by the token's place on axis 0, the next

@@ -4,82 +4,294 @@
 //   g = dy * gamma,  xhat = (s - mu) rstd,  ds = rstd (g - mean(g) - xhat mean(g xhat)) (+ dsum)
 //   dgamma = sum over rows of dy * xhat,  dbeta = sum over rows of dy
 // Statistics, sums and parameter gradients are fp32 whatever the tensors' type.
+// Bound by memory, so every tensor is touched once: a row lives in the registers of its TPR threads as NV 16-byte chunks each (mean, then the
+// variance of the differences: two passes over registers, no difference of squares), and the backward pass takes dx and the sums over
+// rows from the same registers, its threads keeping their columns from row to row.
 #include "token_types.h"
 
 namespace {
 
-// a wave per row
+template <typename T, int NV>
+struct Row {
+  uint4 c[NV];
+  template <int TPR>
+  __device__ __forceinline__ void load(const T* row, int t, int C, int vec) {
+#pragma unroll
+    for (int n = 0; n < NV; ++n) c[n] = load_chunk<T>(row, n * TPR + t, C, vec);
+  }
+  __device__ __forceinline__ void get(int n, float (&f)[Elem<T>::PER_CHUNK]) const {
+    T e[Elem<T>::PER_CHUNK];
+    memcpy(e, &c[n], 16);
+#pragma unroll
+    for (int i = 0; i < Elem<T>::PER_CHUNK; ++i) f[i] = to_f32(e[i]);
+  }
+};
+
+// chunk c of a row from floats, rounded to T
 template <typename T>
-__global__ __launch_bounds__(256) void layernorm_fwd_kernel(const T* __restrict__ x, long ldx, const T* __restrict__ res, long ldr,
-                                                            const float* __restrict__ gamma, const float* __restrict__ beta, T* sum,
-                                                            T* __restrict__ y, float* __restrict__ stat, long rows, int C, float eps) {
-  const int lane = threadIdx.x & 63;
-  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
-  const T* s = x + row * ldx;
-  float t = 0.f;
-  if (res) {
-    T* so = sum + row * C;
-    for (int c = lane; c < C; c += 64) {
-      so[c] = from_f32<T>(to_f32(s[c]) + to_f32(res[row * ldr + c]));
-      t += to_f32(so[c]);
-    }
-    s = so;
+__device__ __forceinline__ uint4 round_chunk(const float (&f)[Elem<T>::PER_CHUNK]) {
+  uint4 u;
+  if constexpr (sizeof(T) == 4) {
+    u = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
   } else {
-    for (int c = lane; c < C; c += 64) t += to_f32(s[c]);
+    const uint2 a = tatt_pack_bf16x4(f[0], f[1], f[2], f[3]), b = tatt_pack_bf16x4(f[4], f[5], f[6], f[7]);
+    u = make_uint4(a.x, a.y, b.x, b.y);
   }
-  const float mu = wave_sum(t) / C;
-  float v = 0.f;
-  for (int c = lane; c < C; c += 64) {
-    const float d = to_f32(s[c]) - mu;
-    v += d * d;
-  }
-  const float rstd = rsqrtf(wave_sum(v) / C + eps);
-  if (stat && lane == 0) {
-    stat[2 * row] = mu;
-    stat[2 * row + 1] = rstd;
-  }
-  for (int c = lane; c < C; c += 64) {
-    const float h = (to_f32(s[c]) - mu) * rstd;
-    y[row * C + c] = from_f32<T>((gamma ? h * gamma[c] : h) + (beta ? beta[c] : 0.f));
-  }
+  return u;
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void layernorm_dx_kernel(const T* __restrict__ s, long lds, const T* __restrict__ dy, long lddy,
-                                                           const T* __restrict__ dsum, long ldds, const float* __restrict__ gamma,
-                                                           const float* __restrict__ stat, T* __restrict__ dx, long rows, int C) {
+__device__ __forceinline__ void store_chunk(T* row, int c, int C, int vec, uint4 u) {
+  constexpr int E = Elem<T>::PER_CHUNK;
+  if (vec) {
+    if (c * E < C) *reinterpret_cast<uint4*>(row + c * E) = u;
+  } else {
+    T t[E];
+    memcpy(t, &u, 16);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (c * E + e < C) row[c * E + e] = t[e];
+  }
+}
+
+// the parameters of chunk c (`none` where there are none), zeros behind the row's end
+template <int E>
+__device__ __forceinline__ void load_params(const float* p, int c, int C, float none, float (&f)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) f[e] = c * E + e < C ? (p ? p[c * E + e] : none) : 0.f;
+}
+
+// (a, b) summed over the TPR threads of a row.  TPR = 256: over the workgroup, red = 8 floats of LDS
+template <int TPR>
+__device__ __forceinline__ float2 row_sum(float a, float b, float* red) {
+#pragma unroll
+  for (int o = (TPR > 64 ? 32 : TPR / 2); o > 0; o >>= 1) {
+    a += __shfl_xor(a, o, 64);
+    b += __shfl_xor(b, o, 64);
+  }
+  if constexpr (TPR > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a, red[4 + (threadIdx.x >> 6)] = b;
+    __syncthreads();
+    a = (red[0] + red[1]) + (red[2] + red[3]);
+    b = (red[4] + red[5]) + (red[6] + red[7]);
+  }
+  return make_float2(a, b);
+}
+
+template <typename T, int TPR, int NV>
+__global__ __launch_bounds__(256) void layernorm_fwd_kernel(const T* __restrict__ x, long ldx, const T* __restrict__ res, long ldr,
+                                                            const float* __restrict__ gamma, const float* __restrict__ beta, T* __restrict__ sum,
+                                                            T* __restrict__ y, float* __restrict__ stat, long rows, int C, float eps, int vec) {
+  constexpr int E = Elem<T>::PER_CHUNK, PER = 256 / TPR;
+  __shared__ float red[8];
+  const int t = threadIdx.x % TPR;
+  for (long r0 = (long)blockIdx.x * PER; r0 < rows; r0 += (long)gridDim.x * PER) {
+    const long row = r0 + threadIdx.x / TPR;
+    const bool on = row < rows;
+    const long at = on ? row : rows - 1;
+    Row<T, NV> s;
+    s.template load<TPR>(x + at * ldx, t, C, vec);
+    float f[E], a = 0.f, b = 0.f;
+    if (res) {
+      Row<T, NV> r;
+      r.template load<TPR>(res + at * ldr, t, C, vec);
+      float g[E];
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        s.get(n, f);
+        r.get(n, g);
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] += g[e];
+        s.c[n] = round_chunk<T>(f);
+        if (on) store_chunk<T>(sum + at * C, n * TPR + t, C, vec, s.c[n]);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      s.get(n, f);
+#pragma unroll
+      for (int e = 0; e < E; ++e) a += f[e];
+    }
+    const float mu = row_sum<TPR>(a, 0.f, red).x / C;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      s.get(n, f);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float d = (n * TPR + t) * E + e < C ? f[e] - mu : 0.f;
+        b += d * d;
+      }
+    }
+    const float rstd = rsqrtf(row_sum<TPR>(b, 0.f, red).x / C + eps);
+    if (!on) continue;
+    if (stat && t == 0) *reinterpret_cast<float2*>(stat + 2 * row) = make_float2(mu, rstd);
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      float w[E], z[E];
+      load_params<E>(gamma, n * TPR + t, C, 1.f, w);
+      load_params<E>(beta, n * TPR + t, C, 0.f, z);
+      s.get(n, f);
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = (f[e] - mu) * rstd * w[e] + z[e];
+      store_chunk<T>(y + row * C, n * TPR + t, C, vec, round_chunk<T>(f));
+    }
+  }
+}
+
+// dx, and partial[block][2][C] of (dgamma, dbeta) where PARAMS
+template <typename T, int TPR, int NV, bool PARAMS>
+__global__ __launch_bounds__(256) void layernorm_bwd_kernel(const T* __restrict__ s, long lds, const T* __restrict__ dy, long lddy, const T* __restrict__ dsum,
+                                                            long ldds, const float* __restrict__ gamma, const float* __restrict__ stat,
+                                                            T* __restrict__ dx, float* __restrict__ partial, long rows, int C, int vec) {
+  constexpr int E = Elem<T>::PER_CHUNK, PER = 256 / TPR;
+  __shared__ float red[8];
+  __shared__ float cols[PARAMS && PER > 1 ? 256 * E : 1];  // one chunk of every thread at a time
+  const int t = threadIdx.x % TPR;
+  float dg[NV][E], db[NV][E];
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int e = 0; e < E; ++e) dg[n][e] = db[n][e] = 0.f;
+  for (long r0 = (long)blockIdx.x * PER; r0 < rows; r0 += (long)gridDim.x * PER) {
+    const long row = r0 + threadIdx.x / TPR;
+    const bool on = row < rows;
+    const long at = on ? row : rows - 1;
+    Row<T, NV> x, d;
+    x.template load<TPR>(s + at * lds, t, C, vec);
+    d.template load<TPR>(dy + at * lddy, t, C, vec);
+    const float2 st = *reinterpret_cast<const float2*>(stat + 2 * at);
+    float a = 0.f, b = 0.f, f[E], g[E], w[E];
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      x.get(n, f);
+      d.get(n, g);
+      load_params<E>(gamma, n * TPR + t, C, 1.f, w);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float h = (f[e] - st.x) * st.y;
+        if (PARAMS && on) dg[n][e] += g[e] * h, db[n][e] += g[e];
+        a += g[e] * w[e];
+        b += g[e] * w[e] * h;
+      }
+    }
+    const float2 ab = row_sum<TPR>(a, b, red);
+    a = ab.x / C;
+    b = ab.y / C;
+    if (!on) continue;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      x.get(n, f);
+      d.get(n, g);
+      load_params<E>(gamma, n * TPR + t, C, 1.f, w);
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = st.y * (g[e] * w[e] - a - (f[e] - st.x) * st.y * b);
+      if (dsum) {
+        const uint4 u = load_chunk<T>(dsum + row * ldds, n * TPR + t, C, vec);
+        T r[E];
+        memcpy(r, &u, 16);
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] += to_f32(r[e]);
+      }
+      store_chunk<T>(dx + row * C, n * TPR + t, C, vec, round_chunk<T>(f));
+    }
+  }
+  if constexpr (PARAMS) {
+    float* p = partial + (long)blockIdx.x * 2 * C;
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        if constexpr (PER > 1) {  // the rows of a pass, in order
+          __syncthreads();
+#pragma unroll
+          for (int e = 0; e < E; ++e) cols[e * 256 + threadIdx.x] = which ? db[n][e] : dg[n][e];
+          __syncthreads();
+          for (int i = threadIdx.x; i < TPR * E; i += 256) {
+            const int c = (n * TPR + i / E) * E + i % E;
+            float v = 0.f;
+#pragma unroll
+            for (int r = 0; r < PER; ++r) v += cols[(i % E) * 256 + r * TPR + i / E];
+            if (c < C) p[which * C + c] = v;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const int c = (n * TPR + t) * E + e;
+            if (c < C) p[which * C + c] = which ? db[n][e] : dg[n][e];
+          }
+        }
+      }
+  }
+}
+
+// ---- rows too wide for the registers of a workgroup: a wave per row, read again for each of its sums ---------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void layernorm_fwd_wide(const T* __restrict__ x, long ldx, const T* __restrict__ res, long ldr,
+                                                          const float* __restrict__ gamma, const float* __restrict__ beta, T* sum, T* __restrict__ y,
+                                                          float* __restrict__ stat, long rows, int C, float eps) {
   const int lane = threadIdx.x & 63;
-  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
-  const float mu = stat[2 * row], rstd = stat[2 * row + 1];
-  float a = 0.f, b = 0.f;
-  for (int c = lane; c < C; c += 64) {
-    const float g = to_f32(dy[row * lddy + c]) * (gamma ? gamma[c] : 1.f), h = (to_f32(s[row * lds + c]) - mu) * rstd;
-    a += g;
-    b += g * h;
-  }
-  a = wave_sum(a) / C;
-  b = wave_sum(b) / C;
-  for (int c = lane; c < C; c += 64) {
-    const float g = to_f32(dy[row * lddy + c]) * (gamma ? gamma[c] : 1.f), h = (to_f32(s[row * lds + c]) - mu) * rstd;
-    const float d = rstd * (g - a - h * b);
-    dx[row * C + c] = from_f32<T>(dsum ? d + to_f32(dsum[row * ldds + c]) : d);
+  for (long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (long)gridDim.x * 4) {
+    const T* s = x + row * ldx;
+    float t = 0.f;
+    if (res) {
+      T* so = sum + row * C;
+      for (int c = lane; c < C; c += 64) {
+        so[c] = from_f32<T>(to_f32(s[c]) + to_f32(res[row * ldr + c]));
+        t += to_f32(so[c]);
+      }
+      s = so;
+    } else {
+      for (int c = lane; c < C; c += 64) t += to_f32(s[c]);
+    }
+    const float mu = wave_sum(t) / C;
+    float v = 0.f;
+    for (int c = lane; c < C; c += 64) {
+      const float d = to_f32(s[c]) - mu;
+      v += d * d;
+    }
+    const float rstd = rsqrtf(wave_sum(v) / C + eps);
+    if (stat && lane == 0) {
+      stat[2 * row] = mu;
+      stat[2 * row + 1] = rstd;
+    }
+    for (int c = lane; c < C; c += 64) {
+      const float h = (to_f32(s[c]) - mu) * rstd;
+      y[row * C + c] = from_f32<T>((gamma ? h * gamma[c] : h) + (beta ? beta[c] : 0.f));
+    }
   }
 }
 
-// partial[blk][2][C]: one thread per column walks the block's rows
-constexpr int MAX_BLOCKS = 512;
+template <typename T>
+__global__ __launch_bounds__(256) void layernorm_dx_wide(const T* __restrict__ s, long lds, const T* __restrict__ dy, long lddy, const T* __restrict__ dsum,
+                                                         long ldds, const float* __restrict__ gamma, const float* __restrict__ stat, T* __restrict__ dx,
+                                                         long rows, int C) {
+  const int lane = threadIdx.x & 63;
+  for (long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (long)gridDim.x * 4) {
+    const float mu = stat[2 * row], rstd = stat[2 * row + 1];
+    float a = 0.f, b = 0.f;
+    for (int c = lane; c < C; c += 64) {
+      const float g = to_f32(dy[row * lddy + c]) * (gamma ? gamma[c] : 1.f), h = (to_f32(s[row * lds + c]) - mu) * rstd;
+      a += g;
+      b += g * h;
+    }
+    a = wave_sum(a) / C;
+    b = wave_sum(b) / C;
+    for (int c = lane; c < C; c += 64) {
+      const float g = to_f32(dy[row * lddy + c]) * (gamma ? gamma[c] : 1.f), h = (to_f32(s[row * lds + c]) - mu) * rstd;
+      const float d = rstd * (g - a - h * b);
+      dx[row * C + c] = from_f32<T>(dsum ? d + to_f32(dsum[row * ldds + c]) : d);
+    }
+  }
+}
 
 template <typename T>
-__global__ __launch_bounds__(256) void layernorm_param_kernel(const T* __restrict__ s, long lds, const T* __restrict__ dy, long lddy,
-                                                              const float* __restrict__ stat, float* __restrict__ partial, long rows,
-                                                              int C, long rows_per_block) {
+__global__ __launch_bounds__(256) void layernorm_params_wide(const T* __restrict__ s, long lds, const T* __restrict__ dy, long lddy,
+                                                             const float* __restrict__ stat, float* __restrict__ partial, long rows, int C) {
   const int c = blockIdx.y * 256 + threadIdx.x;
   if (c >= C) return;
-  const long r0 = blockIdx.x * rows_per_block, r1 = min(rows, r0 + rows_per_block);
   float dg = 0.f, db = 0.f;
-  for (long r = r0; r < r1; ++r) {
+  for (long r = blockIdx.x; r < rows; r += gridDim.x) {
     const float d = to_f32(dy[r * lddy + c]);
     dg += d * ((to_f32(s[r * lds + c]) - stat[2 * r]) * stat[2 * r + 1]);
     db += d;
@@ -88,8 +300,9 @@ __global__ __launch_bounds__(256) void layernorm_param_kernel(const T* __restric
   partial[(blockIdx.x * 2L + 1) * C + c] = db;
 }
 
-__global__ __launch_bounds__(256) void layernorm_param_final(const float* __restrict__ partial, int nblk, int C,
-                                                             float* __restrict__ dgamma, float* __restrict__ dbeta) {
+// partial[block][2][C] -> dgamma, dbeta, in block order
+__global__ __launch_bounds__(256) void layernorm_params_final(const float* __restrict__ partial, int nblk, int C,
+                                                              float* __restrict__ dgamma, float* __restrict__ dbeta) {
   __shared__ float red[256];
   const int c = blockIdx.x * 16 + (threadIdx.x & 15);
   float* dst = blockIdx.y ? dbeta : dgamma;
@@ -97,41 +310,98 @@ __global__ __launch_bounds__(256) void layernorm_param_final(const float* __rest
   if (threadIdx.x < 16 && c < C && dst) dst[c] = v;
 }
 
+// how a row of C elements is held: threads of a row and 16-byte chunks of a thread (0: by none, the wide kernels)
+struct Held {
+  int tpr, nv;
+};
+Held held(int C, int per_chunk) {
+  const int chunks = cdiv(C, per_chunk);
+  if (chunks <= 8) return {8, 1};
+  if (chunks <= 16) return {16, 1};
+  if (chunks <= 32) return {32, 1};
+  if (chunks <= 64) return {64, 1};
+  if (chunks <= 128) return {64, 2};
+  if (chunks <= 256) return {64, 4};
+  if (chunks <= 512) return {64, 8};
+  if (chunks <= 1024) return {256, 4};
+  if (chunks <= 2048) return {256, 8};
+  return {0, 0};
+}
+#define TATT_DISPATCH_HELD(h, ...)                                              \
+  do {                                                                          \
+    if ((h).tpr == 8) { constexpr int TPR = 8, NV = 1; __VA_ARGS__ }            \
+    else if ((h).tpr == 16) { constexpr int TPR = 16, NV = 1; __VA_ARGS__ }     \
+    else if ((h).tpr == 32) { constexpr int TPR = 32, NV = 1; __VA_ARGS__ }     \
+    else if ((h).tpr == 64 && (h).nv == 1) { constexpr int TPR = 64, NV = 1; __VA_ARGS__ } \
+    else if ((h).tpr == 64 && (h).nv == 2) { constexpr int TPR = 64, NV = 2; __VA_ARGS__ } \
+    else if ((h).tpr == 64 && (h).nv == 4) { constexpr int TPR = 64, NV = 4; __VA_ARGS__ } \
+    else if ((h).tpr == 64) { constexpr int TPR = 64, NV = 8; __VA_ARGS__ }     \
+    else if ((h).nv == 4) { constexpr int TPR = 256, NV = 4; __VA_ARGS__ }      \
+    else { constexpr int TPR = 256, NV = 8; __VA_ARGS__ }                       \
+  } while (0)
+
+// workgroups of the backward pass: each leaves 2 C partial sums, so no more than fill the chip (1024; 512 where a thread's columns take most of its registers)
+int bwd_blocks(long rows, int C, int dtype) {
+  const Held h = held(C, dtype == TATT_T_BF16 ? 8 : 4);
+  const long need = h.tpr ? (rows + 256 / h.tpr - 1) / (256 / h.tpr) : rows, most = h.tpr && h.nv <= 2 ? 1024 : 512;
+  return (int)(need < most ? need : most);
+}
+
+constexpr long MAX_GRID = 1 << 16;  // workgroups of the forward pass: more rows go round
+
+bool lined_up(const void* p, long ld, int size) { return !p || (((uintptr_t)p & 15) == 0 && ld * size % 16 == 0); }
+
 }  // namespace
 
 extern "C" {
 
 int tatt_layernorm_fwd(const void* x, long ldx, const void* res, long ldr, const float* gamma, const float* beta, void* sum, void* y,
                        float* stat, long rows, int C, float eps, int dtype, hipStream_t st) {
-  TATT_CHECK_ARG(x && y && rows > 0 && C > 0 && ldx >= C && (!res || (sum && ldr >= C)), "tatt_layernorm_fwd: bad arguments (rows %ld, C %d)", rows, C);
+  TATT_CHECK_ARG(x && y && rows > 0 && C > 0 && (ldx >= C || ldx == 0) && (!res || (sum && (ldr >= C || ldr == 0))), "tatt_layernorm_fwd: bad arguments (rows %ld, C %d)", rows, C);
   TATT_CHECK_ARG(dtype == TATT_T_F32 || dtype == TATT_T_BF16, "tatt_layernorm_fwd: unknown element type %d", dtype);
-  TATT_CHECK_ARG(rows <= (1L << 32), "tatt_layernorm_fwd: more than 2^32 rows");
-  TATT_DISPATCH_TYPE(dtype, hipLaunchKernelGGL(layernorm_fwd_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, (const T*)x, ldx,
-                                               (const T*)res, ldr, gamma, beta, (T*)sum, (T*)y, stat, rows, C, eps););
+  TATT_CHECK_ARG(((uintptr_t)stat & 7) == 0, "tatt_layernorm_fwd: stat is not 8-byte aligned");
+  const int size = dtype == TATT_T_BF16 ? 2 : 4;
+  const int vec = C * size % 16 == 0 && lined_up(x, ldx, size) && lined_up(res, ldr, size) && lined_up(sum, C, size) && lined_up(y, C, size);
+  const Held h = held(C, 16 / size);
+  const int per = h.tpr ? 256 / h.tpr : 4;
+  const long need = (rows + per - 1) / per;
+  const unsigned n = (unsigned)(need < MAX_GRID ? need : MAX_GRID);
+  TATT_DISPATCH_TYPE(
+      dtype, if (!h.tpr) hipLaunchKernelGGL(layernorm_fwd_wide<T>, dim3(n), dim3(256), 0, st, (const T*)x, ldx, (const T*)res, ldr, gamma, beta, (T*)sum,
+                                            (T*)y, stat, rows, C, eps);
+      else TATT_DISPATCH_HELD(h, hipLaunchKernelGGL((layernorm_fwd_kernel<T, TPR, NV>), dim3(n), dim3(256), 0, st, (const T*)x, ldx, (const T*)res, ldr,
+                                                    gamma, beta, (T*)sum, (T*)y, stat, rows, C, eps, vec);););
   TATT_LAUNCH_CHECK("layernorm_fwd");
   return TATT_OK;
 }
 
-size_t tatt_layernorm_workspace(long rows, int C) { return (size_t)(rows < MAX_BLOCKS ? rows : MAX_BLOCKS) * 2 * C; }
+size_t tatt_layernorm_workspace(long rows, int C, int dtype) { return rows > 0 && C > 0 ? (size_t)bwd_blocks(rows, C, dtype) * 2 * C : 0; }
 
 int tatt_layernorm_bwd(const void* s, long lds, const void* dy, long lddy, const void* dsum, long ldds, const float* gamma,
                        const float* stat, void* dx, float* dgamma, float* dbeta, long rows, int C, int dtype, float* workspace,
                        hipStream_t st) {
-  TATT_CHECK_ARG(s && dy && stat && dx && rows > 0 && C > 0 && lds >= C && lddy >= C && (!dsum || ldds >= C), "tatt_layernorm_bwd: bad arguments (rows %ld, C %d)", rows, C);
+  TATT_CHECK_ARG(s && dy && stat && dx && rows > 0 && C > 0 && (lds >= C || lds == 0) && (lddy >= C || lddy == 0) && (!dsum || ldds >= C || ldds == 0),
+                 "tatt_layernorm_bwd: bad arguments (rows %ld, C %d)", rows, C);
   TATT_CHECK_ARG(dtype == TATT_T_F32 || dtype == TATT_T_BF16, "tatt_layernorm_bwd: unknown element type %d", dtype);
   TATT_CHECK_ARG(workspace || (!dgamma && !dbeta), "tatt_layernorm_bwd: parameter gradients need tatt_layernorm_workspace floats");
-  TATT_CHECK_ARG(rows <= (1L << 32), "tatt_layernorm_bwd: more than 2^32 rows");
-  TATT_DISPATCH_TYPE(dtype, hipLaunchKernelGGL(layernorm_dx_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, (const T*)s, lds,
-                                               (const T*)dy, lddy, (const T*)dsum, ldds, gamma, stat, (T*)dx, rows, C););
-  TATT_LAUNCH_CHECK("layernorm_dx");
-  if (dgamma || dbeta) {
-    const int nblk = (int)(rows < MAX_BLOCKS ? rows : MAX_BLOCKS);
-    const long per = (rows + nblk - 1) / nblk;
-    TATT_DISPATCH_TYPE(dtype, hipLaunchKernelGGL(layernorm_param_kernel<T>, dim3(nblk, cdiv(C, 256)), dim3(256), 0, st, (const T*)s, lds,
-                                                 (const T*)dy, lddy, stat, workspace, rows, C, per););
-    TATT_LAUNCH_CHECK("layernorm_param");
-    hipLaunchKernelGGL(layernorm_param_final, dim3(cdiv(C, 16), 2), dim3(256), 0, st, workspace, nblk, C, dgamma, dbeta);
-    TATT_LAUNCH_CHECK("layernorm_param_final");
+  TATT_CHECK_ARG(((uintptr_t)stat & 7) == 0, "tatt_layernorm_bwd: stat is not 8-byte aligned");
+  const int size = dtype == TATT_T_BF16 ? 2 : 4, params = dgamma || dbeta, n = bwd_blocks(rows, C, dtype);
+  const int vec = C * size % 16 == 0 && lined_up(s, lds, size) && lined_up(dy, lddy, size) && lined_up(dsum, ldds, size) && lined_up(dx, C, size);
+  const Held h = held(C, 16 / size);
+  TATT_DISPATCH_TYPE(
+      dtype, if (!h.tpr) {
+        hipLaunchKernelGGL(layernorm_dx_wide<T>, dim3((unsigned)((rows + 3) / 4 < MAX_GRID ? (rows + 3) / 4 : MAX_GRID)), dim3(256), 0, st, (const T*)s, lds,
+                           (const T*)dy, lddy, (const T*)dsum, ldds, gamma, stat, (T*)dx, rows, C);
+        if (params)
+          hipLaunchKernelGGL(layernorm_params_wide<T>, dim3(n, cdiv(C, 256)), dim3(256), 0, st, (const T*)s, lds, (const T*)dy, lddy, stat, workspace, rows, C);
+      } else if (params) TATT_DISPATCH_HELD(h, hipLaunchKernelGGL((layernorm_bwd_kernel<T, TPR, NV, true>), dim3(n), dim3(256), 0, st, (const T*)s, lds,
+                                                                  (const T*)dy, lddy, (const T*)dsum, ldds, gamma, stat, (T*)dx, workspace, rows, C, vec););
+      else TATT_DISPATCH_HELD(h, hipLaunchKernelGGL((layernorm_bwd_kernel<T, TPR, NV, false>), dim3(n), dim3(256), 0, st, (const T*)s, lds, (const T*)dy, lddy,
+                                                    (const T*)dsum, ldds, gamma, stat, (T*)dx, workspace, rows, C, vec);););
+  TATT_LAUNCH_CHECK("layernorm_bwd");
+  if (params) {
+    hipLaunchKernelGGL(layernorm_params_final, dim3(cdiv(C, 16), 2), dim3(256), 0, st, workspace, n, C, dgamma, dbeta);
+    TATT_LAUNCH_CHECK("layernorm_params_final");
   }
   return TATT_OK;
 }

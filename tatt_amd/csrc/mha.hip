@@ -49,22 +49,6 @@ __device__ __forceinline__ Where where(const MhaArgs& a) {
   return w;
 }
 
-// chunk `c` of a row of D elements, zeros behind its end
-template <typename T>
-__device__ __forceinline__ uint4 load_chunk(const T* row, int c, int D, int vec) {
-  constexpr int E = Elem<T>::PER_CHUNK;
-  uint4 r = make_uint4(0, 0, 0, 0);
-  if (vec) {
-    if (c * E < D) r = *reinterpret_cast<const uint4*>(row + c * E);
-  } else {
-    T t[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) t[e] = c * E + e < D ? row[c * E + e] : from_f32<T>(0.f);
-    memcpy(&r, t, 16);
-  }
-  return r;
-}
-
 // element offset of row r (= query * G + head of the group) of a tensor with these token / head strides
 __device__ __forceinline__ long row_offset(int r, int G, long sl, long sh) {
   if (G == 1) return r * sl;

@@ -10,25 +10,6 @@
 #pragma once
 #include "token_types.h"
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
-template <typename T>
-struct Elem;
-
-template <>
-struct Elem<bf16_t> {
-  typedef bf16x8 Frag;                 // 8 contraction places of one lane
-  static constexpr int PER_CHUNK = 8;  // elements of 16 bytes
-  static constexpr int STEP = 16;      // contraction places of an MFMA step (both lane halves)
-};
-template <>
-struct Elem<float> {
-  typedef f32x4 Frag;
-  static constexpr int PER_CHUNK = 4;
-  static constexpr int STEP = 8;
-};
-
 __device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mma(f32x4 a, f32x4 b, f32x16 c) {
 #pragma unroll

@@ -21,6 +21,12 @@ _CT = {
 }
 
 
+def current_stream(device: int | None = None) -> int:
+    """The current stream of a device (default: the current one) as the C ABI takes it.  torch.cuda.current_stream() builds a Stream object
+    for the same number: 2.7 us, against 0.3 us here."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice() if device is None else device)
+
+
 def parse_header(path: str = HEADER_PATH):
     """-> {name: (restype, [(argtype, argname), ...])} for every declaration in the header."""
     txt = open(path).read()
@@ -63,7 +69,7 @@ class _Lib:
         def call(*args):
             conv = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
             if takes_stream and len(conv) == nargs - 1:
-                conv.append(torch.cuda.current_stream().cuda_stream)
+                conv.append(current_stream())
             rc = fn(*conv)
             if is_status and rc != 0:
                 raise RuntimeError(f"{name} failed ({rc}): {self.cdll.tatt_last_error().decode()}")

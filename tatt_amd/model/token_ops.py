@@ -13,33 +13,40 @@ import ctypes
 import torch
 from torch.autograd.function import once_differentiable
 
-from ..lib import lib
+from ..lib import current_stream, lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _POS_TYPES = {torch.int64: 0, torch.int32: 1, torch.float32: 2}
 _L2, _L3, _L9, _L15 = (ctypes.c_long * n for n in (2, 3, 9, 15))
 
 
-def _check(what, *tensors):
+def _check(what, t0, *tensors):
     """The tensors' common element type (as the C ABI's number); raises for what the kernels do not take."""
-    t0 = tensors[0]
+    dtype, device = t0.dtype, t0.device
+    if device.type != "cuda":
+        raise RuntimeError(f"tatt_amd {what} runs on the GPU only (no CPU fallback)")
     for t in tensors:
-        if not t.is_cuda:
-            raise RuntimeError(f"tatt_amd {what} runs on the GPU only (no CPU fallback)")
-        if t.dtype != t0.dtype or t.device != t0.device:
-            raise RuntimeError(f"tatt_amd {what}: tensors of one type on one device expected, got {t0.dtype} on {t0.device} and {t.dtype} on {t.device}")
-    if t0.dtype not in _DTYPES:
-        raise NotImplementedError(f"tatt_amd {what}: float32 or bfloat16 tensors, got {t0.dtype}")
-    return _DTYPES[t0.dtype]
+        if t is not None and (t.dtype != dtype or t.device != device):
+            raise RuntimeError(f"tatt_amd {what}: tensors of one type on one device expected, got {dtype} on {device} and {t.dtype} on {t.device}")
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise NotImplementedError(f"tatt_amd {what}: float32 or bfloat16 tensors, got {dtype}")
+    return code
 
 
-def _call(t, name, *args):
-    """The C entry point on the current stream of t's device."""
-    fn = getattr(lib(), name)
-    if t.device.index != torch.cuda.current_device():
-        with torch.cuda.device(t.device):
-            return fn(*args)
-    return fn(*args)
+def _call(name, device, *args):
+    """A C entry point, tensors given as pointers, on the current stream of `device`."""
+    L, index = lib(), device.index
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return _call(name, device, *args)
+    rc = getattr(L.cdll, name)(*args, current_stream(index))
+    if rc:
+        raise RuntimeError(f"{name} failed ({rc}): {L.cdll.tatt_last_error().decode()}")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _rows(t):
@@ -51,7 +58,7 @@ def _rows(t):
 def _matrix(t):
     """(t as rows, elements between rows): any leading dimensions that one stride covers, else a contiguous copy."""
     C = t.shape[-1]
-    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= C:
+    if t.dim() == 2 and t.stride(1) == 1 and (t.stride(0) >= C or t.stride(0) == 0):
         return t, t.stride(0)
     return t.contiguous(), C
 
@@ -65,7 +72,7 @@ def _parameters(what, x, weight, bias):
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None, need_stat=True):
     """-> (y, sum, stat): y = LayerNorm(sum) over the last dimension, sum = x + residual in x's type (x itself without a residual), stat
     [rows, 2] fp32 = (mean, 1/sqrt(var + eps)) for layer_norm_backward (None unless need_stat)."""
-    dtype = _check("layer_norm", x, *(() if residual is None else (residual,)))
+    dtype = _check("layer_norm", x, residual)
     if x.dim() == 0 or x.shape[-1] == 0:
         raise RuntimeError("tatt_amd layer_norm: the last dimension is empty")
     if residual is not None and residual.shape != x.shape:
@@ -79,18 +86,19 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None, need_
     if R:
         xm, ldx = _matrix(x)
         rm, ldr = (None, 0) if residual is None else _matrix(residual)
-        _call(x, "layernorm_fwd", xm, ldx, rm, ldr, weight, bias, None if residual is None else s, y, stat, R, C, eps, dtype)
+        _call("tatt_layernorm_fwd", x.device, xm.data_ptr(), ldx, _ptr(rm), ldr, _ptr(weight), _ptr(bias), None if residual is None else s.data_ptr(),
+              y.data_ptr(), _ptr(stat), R, C, eps, dtype)
     return y, s, stat
 
 
 def layer_norm_backward(dy, s, weight, stat, dsum=None, need_params=True):
     """-> (ds, dweight, dbias) of layer_norm_forward: ds = the gradient of the sum (x's and the residual's alike), with dsum, what reaches the
     sum by other ways, added; dweight and dbias fp32 (None unless need_params)."""
-    dtype = _check("layer_norm", s, dy, *(() if dsum is None else (dsum,)))
+    dtype = _check("layer_norm", s, dy, dsum)
     _parameters("layer_norm", s, weight, None)
     C = s.shape[-1]
     R = s.numel() // C
-    if dy.shape != s.shape or (dsum is not None and dsum.shape != s.shape) or stat.shape != (R, 2) or stat.dtype != torch.float32 or not stat.is_contiguous():
+    if dy.shape != s.shape or (dsum is not None and dsum.shape != s.shape) or stat.shape != (R, 2) or stat.dtype != torch.float32 or stat.device != s.device or not stat.is_contiguous():
         raise RuntimeError("tatt_amd layer_norm_backward: dy and dsum have the shape of the sum, stat is layer_norm_forward's")
     ds = torch.empty(s.shape, dtype=s.dtype, device=s.device)
     dw, db = (torch.empty(2, C, dtype=torch.float32, device=s.device) if R else torch.zeros(2, C, device=s.device)).unbind() if need_params else (None, None)
@@ -98,8 +106,9 @@ def layer_norm_backward(dy, s, weight, stat, dsum=None, need_params=True):
         sm, lds = _matrix(s)
         dym, lddy = _matrix(dy)
         dm, ldd = (None, 0) if dsum is None else _matrix(dsum)
-        ws = torch.empty(lib().layernorm_workspace(R, C), dtype=torch.float32, device=s.device) if need_params else None
-        _call(s, "layernorm_bwd", sm, lds, dym, lddy, dm, ldd, weight, stat, ds, dw, db, R, C, dtype, ws)
+        ws = torch.empty(lib().cdll.tatt_layernorm_workspace(R, C, dtype), dtype=torch.float32, device=s.device) if need_params else None
+        _call("tatt_layernorm_bwd", s.device, sm.data_ptr(), lds, dym.data_ptr(), lddy, _ptr(dm), ldd, _ptr(weight), stat.data_ptr(), ds.data_ptr(),
+              _ptr(dw), _ptr(db), R, C, dtype, _ptr(ws))
     return ds, dw, db
 
 
@@ -139,7 +148,7 @@ def rotary_frequencies(sections, base=10000.0, device="cuda"):
 
 def rotate(q, k, positions, freqs, sections, interleaved=False, inverse=False):
     """`rotary` without autograd; inverse=True turns back (its backward pass)."""
-    dtype = _check("rotary", q, *(() if k is None else (k,)))
+    dtype = _check("rotary", q, k)
     n = len(sections)
     if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
         raise RuntimeError("tatt_amd rotary: q [B, L, H, D] and k [B, L, Hk, D] expected")
@@ -158,8 +167,9 @@ def rotate(q, k, positions, freqs, sections, interleaved=False, inverse=False):
         q, k = _rows(q), None if k is None or not k.numel() else _rows(k)
         sp = positions.stride()
         pos_strides = _L3(sp[0] if len(sp) == 3 and positions.shape[0] > 1 else 0, sp[-2], sp[-1])
-        _call(q, "rotary", q, _L3(*q.stride()[:3]), qo, H, k, None if k is None else _L3(*k.stride()[:3]), ko, 0 if k is None else k.shape[2],
-              positions, _POS_TYPES[positions.dtype], pos_strides, freqs, (ctypes.c_int * n)(*sections), n, B, L, D, bool(interleaved), bool(inverse), dtype)
+        _call("tatt_rotary", q.device, q.data_ptr(), _L3(*q.stride()[:3]), qo.data_ptr(), H, _ptr(k), None if k is None else _L3(*k.stride()[:3]), _ptr(ko),
+              0 if k is None else k.shape[2], positions.data_ptr(), _POS_TYPES[positions.dtype], pos_strides, freqs.data_ptr(),
+              (ctypes.c_int * n)(*sections), n, B, L, D, bool(interleaved), bool(inverse), dtype)
     return qo, ko
 
 
@@ -220,11 +230,11 @@ def attention_forward(q, k, v, key_padding_mask=None, causal=False, scale=None, 
     q, k, v = _rows(q), _rows(k), _rows(v)
     out = torch.empty(B, Lq, H, D, dtype=q.dtype, device=q.device)
     lse = torch.empty(B, H, Lq, dtype=torch.float32, device=q.device) if need_lse else None
-    n = lib().mha_fwd_workspace(*dims, dtype)
+    n = lib().cdll.tatt_mha_fwd_workspace(*dims, dtype)
     ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
     mask_strides = None if key_padding_mask is None else _L2(*key_padding_mask.stride())
-    _call(q, "mha_fwd", q, k, v, _L9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]), key_padding_mask, mask_strides, out, lse, *dims,
-          scale, bool(causal), dtype, ws)
+    _call("tatt_mha_fwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), _L9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]),
+          _ptr(key_padding_mask), mask_strides, out.data_ptr(), _ptr(lse), *dims, scale, bool(causal), dtype, _ptr(ws))
     return out, lse
 
 
@@ -233,17 +243,18 @@ def attention_backward(dout, q, k, v, out, lse, key_padding_mask=None, causal=Fa
     dtype, dims, scale = _attention_args(q, k, v, key_padding_mask, scale)
     _check("attention", q, out, dout)
     B, Lq, Lk, H, Hk, D = dims
-    if out.shape != q.shape or dout.shape != q.shape or lse.shape != (B, H, Lq) or lse.dtype != torch.float32 or not lse.is_contiguous():
+    if out.shape != q.shape or dout.shape != q.shape or lse.shape != (B, H, Lq) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
         raise RuntimeError("tatt_amd attention_backward: out and dout have the shape of q, lse is attention_forward's")
     if B == 0 or Lq == 0 or Lk == 0:
         return q.new_zeros(q.shape), k.new_zeros(k.shape), v.new_zeros(v.shape)
     q, k, v, out, dout = _rows(q), _rows(k), _rows(v), _rows(out), _rows(dout)
     dq = torch.empty(B, Lq, H, D, dtype=q.dtype, device=q.device)
     dk, dv = (torch.empty(B, Lk, Hk, D, dtype=q.dtype, device=q.device) for _ in range(2))
-    ws = torch.empty(lib().mha_bwd_workspace(*dims, dtype), dtype=torch.float32, device=q.device)
+    ws = torch.empty(lib().cdll.tatt_mha_bwd_workspace(*dims, dtype), dtype=torch.float32, device=q.device)
     mask_strides = None if key_padding_mask is None else _L2(*key_padding_mask.stride())
-    _call(q, "mha_bwd", q, k, v, _L15(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *dout.stride()[:3]),
-          key_padding_mask, mask_strides, out, dout, lse, dq, dk, dv, *dims, scale, bool(causal), dtype, ws)
+    _call("tatt_mha_bwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+          _L15(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *dout.stride()[:3]), _ptr(key_padding_mask), mask_strides,
+          out.data_ptr(), dout.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *dims, scale, bool(causal), dtype, ws.data_ptr())
     return dq, dk, dv
 
 
