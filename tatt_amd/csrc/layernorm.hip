@@ -54,14 +54,25 @@ __device__ __forceinline__ void store_chunk(T* row, int c, int C, int vec, uint4
   }
 }
 
+// whether element e of chunk c is within the row (`vec`: chunks are whole)
+__device__ __forceinline__ bool within(int c, int e, int E, int C, int vec) { return vec ? c * E < C : c * E + e < C; }
+
 // the parameters of chunk c (`none` where there are none), zeros behind the row's end
 template <int E>
-__device__ __forceinline__ void load_params(const float* p, int c, int C, float none, float (&f)[E]) {
+__device__ __forceinline__ void load_params(const float* p, int c, int C, float none, int vec, float (&f)[E]) {
+  if (p && vec) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) f[e] = c * E + e < C ? (p ? p[c * E + e] : none) : 0.f;
+    for (int e = 0; e < E; e += 4) {
+      const float4 v = c * E < C ? *reinterpret_cast<const float4*>(p + c * E + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+      f[e] = v.x, f[e + 1] = v.y, f[e + 2] = v.z, f[e + 3] = v.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) f[e] = within(c, e, E, C, vec) ? (p ? p[c * E + e] : none) : 0.f;
 }
 
-// (a, b) summed over the TPR threads of a row.  TPR = 256: over the workgroup, red = 8 floats of LDS
+// (a, b) summed over the TPR threads of a row.  TPR >= 256: over the workgroup, red = 32 floats of LDS
 template <int TPR>
 __device__ __forceinline__ float2 row_sum(float a, float b, float* red) {
 #pragma unroll
@@ -71,20 +82,24 @@ __device__ __forceinline__ float2 row_sum(float a, float b, float* red) {
   }
   if constexpr (TPR > 64) {
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a, red[4 + (threadIdx.x >> 6)] = b;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a, red[16 + (threadIdx.x >> 6)] = b;
     __syncthreads();
-    a = (red[0] + red[1]) + (red[2] + red[3]);
-    b = (red[4] + red[5]) + (red[6] + red[7]);
+    a = b = 0.f;
+#pragma unroll
+    for (int i = 0; i < TPR / 64; ++i) a += red[i], b += red[16 + i];
   }
   return make_float2(a, b);
 }
 
-template <typename T, int TPR, int NV>
-__global__ __launch_bounds__(256) void layernorm_fwd_kernel(const T* __restrict__ x, long ldx, const T* __restrict__ res, long ldr,
+// threads of a workgroup
+constexpr int block_of(int tpr) { return tpr > 256 ? tpr : 256; }
+
+template <typename T, int TPR, int NV, int vec>
+__global__ __launch_bounds__(block_of(TPR)) void layernorm_fwd_kernel(const T* __restrict__ x, long ldx, const T* __restrict__ res, long ldr,
                                                             const float* __restrict__ gamma, const float* __restrict__ beta, T* __restrict__ sum,
-                                                            T* __restrict__ y, float* __restrict__ stat, long rows, int C, float eps, int vec) {
-  constexpr int E = Elem<T>::PER_CHUNK, PER = 256 / TPR;
-  __shared__ float red[8];
+                                                            T* __restrict__ y, float* __restrict__ stat, long rows, int C, float eps) {
+  constexpr int E = Elem<T>::PER_CHUNK, PER = block_of(TPR) / TPR;
+  __shared__ float red[32];
   const int t = threadIdx.x % TPR;
   for (long r0 = (long)blockIdx.x * PER; r0 < rows; r0 += (long)gridDim.x * PER) {
     const long row = r0 + threadIdx.x / TPR;
@@ -119,7 +134,7 @@ __global__ __launch_bounds__(256) void layernorm_fwd_kernel(const T* __restrict_
       s.get(n, f);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float d = (n * TPR + t) * E + e < C ? f[e] - mu : 0.f;
+        const float d = within(n * TPR + t, e, E, C, vec) ? f[e] - mu : 0.f;
         b += d * d;
       }
     }
@@ -129,8 +144,8 @@ __global__ __launch_bounds__(256) void layernorm_fwd_kernel(const T* __restrict_
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       float w[E], z[E];
-      load_params<E>(gamma, n * TPR + t, C, 1.f, w);
-      load_params<E>(beta, n * TPR + t, C, 0.f, z);
+      load_params<E>(gamma, n * TPR + t, C, 1.f, vec, w);
+      load_params<E>(beta, n * TPR + t, C, 0.f, vec, z);
       s.get(n, f);
 #pragma unroll
       for (int e = 0; e < E; ++e) f[e] = (f[e] - mu) * rstd * w[e] + z[e];
@@ -140,12 +155,12 @@ __global__ __launch_bounds__(256) void layernorm_fwd_kernel(const T* __restrict_
 }
 
 // dx, and partial[block][2][C] of (dgamma, dbeta) where PARAMS
-template <typename T, int TPR, int NV, bool PARAMS>
-__global__ __launch_bounds__(256) void layernorm_bwd_kernel(const T* __restrict__ s, long lds, const T* __restrict__ dy, long lddy, const T* __restrict__ dsum,
+template <typename T, int TPR, int NV, int vec, bool PARAMS>
+__global__ __launch_bounds__(block_of(TPR)) void layernorm_bwd_kernel(const T* __restrict__ s, long lds, const T* __restrict__ dy, long lddy, const T* __restrict__ dsum,
                                                             long ldds, const float* __restrict__ gamma, const float* __restrict__ stat,
-                                                            T* __restrict__ dx, float* __restrict__ partial, long rows, int C, int vec) {
-  constexpr int E = Elem<T>::PER_CHUNK, PER = 256 / TPR;
-  __shared__ float red[8];
+                                                            T* __restrict__ dx, float* __restrict__ partial, long rows, int C) {
+  constexpr int E = Elem<T>::PER_CHUNK, PER = block_of(TPR) / TPR;
+  __shared__ float red[32];
   __shared__ float cols[PARAMS && PER > 1 ? 256 * E : 1];  // one chunk of every thread at a time
   const int t = threadIdx.x % TPR;
   float dg[NV][E], db[NV][E];
@@ -166,7 +181,7 @@ __global__ __launch_bounds__(256) void layernorm_bwd_kernel(const T* __restrict_
     for (int n = 0; n < NV; ++n) {
       x.get(n, f);
       d.get(n, g);
-      load_params<E>(gamma, n * TPR + t, C, 1.f, w);
+      load_params<E>(gamma, n * TPR + t, C, 1.f, vec, w);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const float h = (f[e] - st.x) * st.y;
@@ -183,7 +198,7 @@ __global__ __launch_bounds__(256) void layernorm_bwd_kernel(const T* __restrict_
     for (int n = 0; n < NV; ++n) {
       x.get(n, f);
       d.get(n, g);
-      load_params<E>(gamma, n * TPR + t, C, 1.f, w);
+      load_params<E>(gamma, n * TPR + t, C, 1.f, vec, w);
 #pragma unroll
       for (int e = 0; e < E; ++e) f[e] = st.y * (g[e] * w[e] - a - (f[e] - st.x) * st.y * b);
       if (dsum) {
@@ -321,29 +336,46 @@ Held held(int C, int per_chunk) {
   if (chunks <= 32) return {32, 1};
   if (chunks <= 64) return {64, 1};
   if (chunks <= 128) return {64, 2};
-  if (chunks <= 256) return {64, 4};
-  if (chunks <= 512) return {64, 8};
-  if (chunks <= 1024) return {256, 4};
-  if (chunks <= 2048) return {256, 8};
+  if (chunks <= 256) return {256, 1};
+  if (chunks <= 512) return {256, 2};
+  if (chunks <= 1024) return {512, 2};
+  if (chunks <= 2048) return {1024, 2};
   return {0, 0};
 }
-#define TATT_DISPATCH_HELD(h, ...)                                              \
-  do {                                                                          \
-    if ((h).tpr == 8) { constexpr int TPR = 8, NV = 1; __VA_ARGS__ }            \
-    else if ((h).tpr == 16) { constexpr int TPR = 16, NV = 1; __VA_ARGS__ }     \
-    else if ((h).tpr == 32) { constexpr int TPR = 32, NV = 1; __VA_ARGS__ }     \
-    else if ((h).tpr == 64 && (h).nv == 1) { constexpr int TPR = 64, NV = 1; __VA_ARGS__ } \
-    else if ((h).tpr == 64 && (h).nv == 2) { constexpr int TPR = 64, NV = 2; __VA_ARGS__ } \
-    else if ((h).tpr == 64 && (h).nv == 4) { constexpr int TPR = 64, NV = 4; __VA_ARGS__ } \
-    else if ((h).tpr == 64) { constexpr int TPR = 64, NV = 8; __VA_ARGS__ }     \
-    else if ((h).nv == 4) { constexpr int TPR = 256, NV = 4; __VA_ARGS__ }      \
-    else { constexpr int TPR = 256, NV = 8; __VA_ARGS__ }                       \
+#define TATT_DISPATCH_HELD(h, ...)                                                           \
+  do {                                                                                       \
+    if ((h).tpr == 8) { constexpr int TPR = 8, NV = 1; __VA_ARGS__ }                         \
+    else if ((h).tpr == 16) { constexpr int TPR = 16, NV = 1; __VA_ARGS__ }                  \
+    else if ((h).tpr == 32) { constexpr int TPR = 32, NV = 1; __VA_ARGS__ }                  \
+    else if ((h).tpr == 64 && (h).nv == 1) { constexpr int TPR = 64, NV = 1; __VA_ARGS__ }   \
+    else if ((h).tpr == 64) { constexpr int TPR = 64, NV = 2; __VA_ARGS__ }                  \
+    else if ((h).tpr == 256 && (h).nv == 1) { constexpr int TPR = 256, NV = 1; __VA_ARGS__ } \
+    else if ((h).tpr == 256) { constexpr int TPR = 256, NV = 2; __VA_ARGS__ }                \
+    else if ((h).tpr == 512) { constexpr int TPR = 512, NV = 2; __VA_ARGS__ }                \
+    else { constexpr int TPR = 1024, NV = 2; __VA_ARGS__ }                                   \
   } while (0)
 
-// workgroups of the backward pass: each leaves 2 C partial sums, so no more than fill the chip (1024; 512 where a thread's columns take most of its registers)
+// one launch, with 16-byte loads or without
+template <typename T, int TPR, int NV>
+void launch_fwd(bool vec, unsigned n, hipStream_t st, const T* x, long ldx, const T* res, long ldr, const float* gamma, const float* beta, T* sum, T* y,
+                float* stat, long rows, int C, float eps) {
+  if (vec)
+    hipLaunchKernelGGL((layernorm_fwd_kernel<T, TPR, NV, 1>), dim3(n), dim3(block_of(TPR)), 0, st, x, ldx, res, ldr, gamma, beta, sum, y, stat, rows, C, eps);
+  else
+    hipLaunchKernelGGL((layernorm_fwd_kernel<T, TPR, NV, 0>), dim3(n), dim3(block_of(TPR)), 0, st, x, ldx, res, ldr, gamma, beta, sum, y, stat, rows, C, eps);
+}
+template <typename T, int TPR, int NV>
+void launch_bwd(bool vec, bool params, unsigned n, hipStream_t st, const T* s, long lds, const T* dy, long lddy, const T* dsum, long ldds, const float* gamma,
+                const float* stat, T* dx, float* partial, long rows, int C) {
+  auto kernel = vec ? (params ? layernorm_bwd_kernel<T, TPR, NV, 1, true> : layernorm_bwd_kernel<T, TPR, NV, 1, false>)
+                    : (params ? layernorm_bwd_kernel<T, TPR, NV, 0, true> : layernorm_bwd_kernel<T, TPR, NV, 0, false>);
+  hipLaunchKernelGGL(kernel, dim3(n), dim3(block_of(TPR)), 0, st, s, lds, dy, lddy, dsum, ldds, gamma, stat, dx, partial, rows, C);
+}
+
+// workgroups of the backward pass: each leaves 2 C partial sums, so no more than fill the chip
 int bwd_blocks(long rows, int C, int dtype) {
   const Held h = held(C, dtype == TATT_T_BF16 ? 8 : 4);
-  const long need = h.tpr ? (rows + 256 / h.tpr - 1) / (256 / h.tpr) : rows, most = h.tpr && h.nv <= 2 ? 1024 : 512;
+  const long per = h.tpr ? block_of(h.tpr) / h.tpr : 1, need = (rows + per - 1) / per, most = h.tpr > 256 ? 512 : 1024;
   return (int)(need < most ? need : most);
 }
 
@@ -361,16 +393,17 @@ int tatt_layernorm_fwd(const void* x, long ldx, const void* res, long ldr, const
   TATT_CHECK_ARG(dtype == TATT_T_F32 || dtype == TATT_T_BF16, "tatt_layernorm_fwd: unknown element type %d", dtype);
   TATT_CHECK_ARG(((uintptr_t)stat & 7) == 0, "tatt_layernorm_fwd: stat is not 8-byte aligned");
   const int size = dtype == TATT_T_BF16 ? 2 : 4;
-  const int vec = C * size % 16 == 0 && lined_up(x, ldx, size) && lined_up(res, ldr, size) && lined_up(sum, C, size) && lined_up(y, C, size);
+  const int vec = C * size % 16 == 0 && lined_up(x, ldx, size) && lined_up(res, ldr, size) && lined_up(sum, C, size) && lined_up(y, C, size) &&
+                  lined_up(gamma, 4, 4) && lined_up(beta, 4, 4);
   const Held h = held(C, 16 / size);
-  const int per = h.tpr ? 256 / h.tpr : 4;
+  const int per = h.tpr ? block_of(h.tpr) / h.tpr : 4;
   const long need = (rows + per - 1) / per;
   const unsigned n = (unsigned)(need < MAX_GRID ? need : MAX_GRID);
   TATT_DISPATCH_TYPE(
       dtype, if (!h.tpr) hipLaunchKernelGGL(layernorm_fwd_wide<T>, dim3(n), dim3(256), 0, st, (const T*)x, ldx, (const T*)res, ldr, gamma, beta, (T*)sum,
                                             (T*)y, stat, rows, C, eps);
-      else TATT_DISPATCH_HELD(h, hipLaunchKernelGGL((layernorm_fwd_kernel<T, TPR, NV>), dim3(n), dim3(256), 0, st, (const T*)x, ldx, (const T*)res, ldr,
-                                                    gamma, beta, (T*)sum, (T*)y, stat, rows, C, eps, vec);););
+      else TATT_DISPATCH_HELD(h, launch_fwd<T, TPR, NV>(vec, n, st, (const T*)x, ldx, (const T*)res, ldr, gamma, beta, (T*)sum, (T*)y, stat, rows, C, eps););
+  );
   TATT_LAUNCH_CHECK("layernorm_fwd");
   return TATT_OK;
 }
@@ -386,7 +419,8 @@ int tatt_layernorm_bwd(const void* s, long lds, const void* dy, long lddy, const
   TATT_CHECK_ARG(workspace || (!dgamma && !dbeta), "tatt_layernorm_bwd: parameter gradients need tatt_layernorm_workspace floats");
   TATT_CHECK_ARG(((uintptr_t)stat & 7) == 0, "tatt_layernorm_bwd: stat is not 8-byte aligned");
   const int size = dtype == TATT_T_BF16 ? 2 : 4, params = dgamma || dbeta, n = bwd_blocks(rows, C, dtype);
-  const int vec = C * size % 16 == 0 && lined_up(s, lds, size) && lined_up(dy, lddy, size) && lined_up(dsum, ldds, size) && lined_up(dx, C, size);
+  const int vec = C * size % 16 == 0 && lined_up(s, lds, size) && lined_up(dy, lddy, size) && lined_up(dsum, ldds, size) && lined_up(dx, C, size) &&
+                  lined_up(gamma, 4, 4);
   const Held h = held(C, 16 / size);
   TATT_DISPATCH_TYPE(
       dtype, if (!h.tpr) {
@@ -394,10 +428,9 @@ int tatt_layernorm_bwd(const void* s, long lds, const void* dy, long lddy, const
                            (const T*)dy, lddy, (const T*)dsum, ldds, gamma, stat, (T*)dx, rows, C);
         if (params)
           hipLaunchKernelGGL(layernorm_params_wide<T>, dim3(n, cdiv(C, 256)), dim3(256), 0, st, (const T*)s, lds, (const T*)dy, lddy, stat, workspace, rows, C);
-      } else if (params) TATT_DISPATCH_HELD(h, hipLaunchKernelGGL((layernorm_bwd_kernel<T, TPR, NV, true>), dim3(n), dim3(256), 0, st, (const T*)s, lds,
-                                                                  (const T*)dy, lddy, (const T*)dsum, ldds, gamma, stat, (T*)dx, workspace, rows, C, vec););
-      else TATT_DISPATCH_HELD(h, hipLaunchKernelGGL((layernorm_bwd_kernel<T, TPR, NV, false>), dim3(n), dim3(256), 0, st, (const T*)s, lds, (const T*)dy, lddy,
-                                                    (const T*)dsum, ldds, gamma, stat, (T*)dx, workspace, rows, C, vec);););
+      } else TATT_DISPATCH_HELD(h, launch_bwd<T, TPR, NV>(vec, params, n, st, (const T*)s, lds, (const T*)dy, lddy, (const T*)dsum, ldds, gamma, stat, (T*)dx,
+                                                          workspace, rows, C););
+  );
   TATT_LAUNCH_CHECK("layernorm_bwd");
   if (params) {
     hipLaunchKernelGGL(layernorm_params_final, dim3(cdiv(C, 16), 2), dim3(256), 0, st, workspace, n, C, dgamma, dbeta);
