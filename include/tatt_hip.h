@@ -365,8 +365,7 @@ int tatt_clip_adam(float* p, const float* g, float* m, float* v, long n, float l
 /* ---- token operators: one transformer layer over image or text tokens of any size -------------------------------------------
  * The interpreter's own layers (tatt_ln_*, tatt_attn_*, tatt_dec_*) are built for 64 channels, 4 heads x 16 and 26 keys; these take any
  * width, lengths and head counts, fp32 or bf16 tensors (`dtype` = TATT_T_F32 / TATT_T_BF16; parameters, statistics and sums fp32).
- * void* tensors are of that type; strides count elements; `strides` arguments are HOST arrays, read during the call.  Tensors may
- * have any element alignment; 16-byte aligned pointers and strides take the wide loads.  No atomics: results are bit-reproducible.
+ * void* tensors are of that type; strides count elements; `strides` arguments are HOST arrays, read during the call.  No atomics: results are bit-reproducible.
  *
  * LayerNorm over C columns (nn.LayerNorm at model/transformer_v2.py:478-482, :827-831, of any width), optionally with the residual sum in front:
  *   s = x + res (stored to sum, contiguous, rounded to the type; res = NULL: s = x), y = (s - mu) rstd gamma + beta (NULL: 1 / 0),
@@ -387,7 +386,8 @@ int tatt_rotary(const void* q, const long* q_strides, void* q_out, int Hq, const
 
 /* Attention (nn.MultiheadAttention's core at model/transformer_v2.py:476, :819, of any size): q [B][Lq][H][D], k / v [B][Lk][Hkv][D], D <= 128, H a
  * multiple of Hkv (query head h reads key head h / (H / Hkv)); strides = HOST array of (batch, token, head) for q, k, v (9 values; the
- * backward call: and out, dout, 15 values).  key_mask (may be NULL): bytes [B][Lk], not 0 = leave the key out, mask_strides (batch, key).  causal: query i
+ * backward call: and out, dout, 15 values); rows of whole 16 bytes at 16-byte aligned places (pad D with zeros, which add nothing), token and
+ * head strides of less than 2^24 bytes.  key_mask (may be NULL): bytes [B][Lk], not 0 = leave the key out, mask_strides (batch, key).  causal: query i
  * sees key j iff j <= i + Lk - Lq.  out contiguous [B][Lq][H][D]; lse [B][H][Lq] = base-2 logarithm of the sum of the
  * exponentials (NULL if no backward call follows).  A row that sees no key gives zeros, lse = +inf, and no gradient.  The backward call recomputes the probabilities from lse; dq, dk, dv contiguous.
  * workspace: tatt_mha_*_workspace floats (0 = may be NULL). */

@@ -1,0 +1,369 @@
+// What the attention kernels (mha_fwd.hip, mha_bwd.hip) share: tiles and matrix-core fragments, the way of a tensor's rows into LDS, the
+// arguments, their checks and the launch plans.
+//
+//   S = log2(e) scale q k^T;  lse_i = log2 sum_j 2^S_ij;  P = 2^(S - lse);  O = P V
+//   delta_i = dO_i . O_i;  dV = P^T dO;  dS = P (dO V^T - delta);  dQ = scale dS K;  dK = scale dS^T Q
+// lse stays in base 2 between the passes: a change of base would round it twice more, and P is off by lse times those roundings.
+// H = G * Hkv query heads: head h reads key head h / G.  The G heads of a key head are rows of the same problem (row = query * G + head), so a
+// single query of G heads fills G rows of a tile, and a key's gradient sums over its heads as it sums over queries.
+// Hidden places: keys whose mask byte is not 0, and, where causal, j > i + Lk - Lq.  A row that sees nothing gives zeros (lse = +inf) and
+// takes no part in any gradient; a masked key's K and V are replaced by zeros on their way into LDS, whatever they hold.
+//
+// Every product is an MFMA of 32x32 outputs whose B operand sits in registers and whose A operand is read from a row-major tile in LDS:
+//   rows(tile) x contraction over the head's dimensions   (scores, dP)          A = 32 tile rows, read as 16-byte chunks
+//   dimensions x contraction over the tile's rows         (O, dQ, dK, dV)       A = the tile transposed
+// The accumulator of the first kind (lane = column, registers = tile rows 8 (i / 4) + 4 half + i % 4) is, register for register, a B operand of
+// the second kind if the contraction visits the tile's rows in that order: no element changes its lane between the two products.
+//   bf16: v_mfma_f32_32x32x16_bf16, a chunk pair (16 dimensions) a step; transposed reads are ds_read_b64_tr_b16 (4 rows x 16 dimensions to 16 lanes)
+//   fp32: v_mfma_f32_32x32x2_f32, four a step (8 dimensions); transposed reads are 4-byte reads along a row
+// Operands are rounded to bf16 only where the tensors are bf16 (P and dS enter their second product in bf16: 2^-9 of a term, the error that the
+// stored result carries anyway); accumulation is fp32.
+#pragma once
+#include "token_types.h"
+
+namespace {
+
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma(f32x4 a, f32x4 b, f32x16 c) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[t], b[t], c, 0, 0, 0);
+  return c;
+}
+
+// accumulator registers [step * n, step * n + n) as the B operand of the transposed product's step (n = 8 bf16, 4 fp32); bf16: rounded to nearest even
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::Frag pack_step(const f32x16& c, int step) {
+  typename Elem<T>::Frag r;
+#pragma unroll
+  for (int j = 0; j < Elem<T>::PER_CHUNK; ++j) {
+    if constexpr (sizeof(T) == 4)
+      r[j] = c[step * 4 + j];
+    else
+      r[j] = (__bf16)c[step * 8 + j];
+  }
+  return r;
+}
+
+// waves a SIMD that the registers are shared out for.  Two (256 registers each) unless what a wave has to hold -- the fragments of its rows, the
+// sums, a tile on its way -- would spill: then one, the sums in the other half of the register file.
+template <typename T>
+constexpr int fwd_waves(int DK) { return sizeof(T) == 4 && DK > 64 ? 1 : 2; }
+template <typename T>
+constexpr int dq_waves(int DK) { return sizeof(T) == 4 && DK >= 64 ? 1 : 2; }
+template <typename T>
+constexpr int dkv_waves(int DK) { return DK > 64 || (sizeof(T) == 4 && DK == 64) ? 1 : 2; }
+
+// head widths the kernels are built for, and the LDS row that holds one
+constexpr int row_width(int DK) { return DK <= 32 ? 32 : DK <= 64 ? 64 : 128; }
+
+// A row-major LDS tile of W elements a row (a power of two, 32 to 128).  The 16-byte chunks of row r are stored at chunk ^ swizzle(r): the 16
+// rows of a chunk column fall into 16 different 16-byte slots of the 256 bytes that LDS serves at once, and so do the chunks that four
+// neighbouring rows of a transposed read take.
+template <typename T, int W>
+struct Tile {
+  static constexpr int NC = W * (int)sizeof(T) / 16;  // chunks of a row: 4, 8, 16 or 32
+  static constexpr int ROW = NC * 16;                 // bytes of a row
+  __device__ __forceinline__ static int swizzle(int r) {
+    if (NC >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+    if (NC == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+    return (r >> 2) & 3;
+  }
+  __device__ __forceinline__ static int offset(int r, int chunk) { return r * ROW + ((chunk ^ swizzle(r)) << 4); }
+
+  // A operand of a row product: lane (row = lane % 32, half) holds chunk 2 step + half of its row
+  __device__ __forceinline__ static typename Elem<T>::Frag rows(const char* tile, int row0, int step, int lane) {
+    return *reinterpret_cast<const typename Elem<T>::Frag*>(tile + row0 * ROW + offset(lane & 31, 2 * step + (lane >> 5)));
+  }
+
+  // A operand of a transposed product: lane (dimension d0 + lane % 32, half) holds the tile rows that accumulator registers of `step` stand for:
+  // fp32: row0 + 8 step + 4 half + j;  bf16: row0 + 16 step + 4 half + {0..3, 8..11}.  d0 and row0 multiples of 32.
+  __device__ __forceinline__ static typename Elem<T>::Frag transposed(const char* tile, int row0, int step, int d0, int lane) {
+    const int half = lane >> 5;
+    if constexpr (sizeof(T) == 4) {
+      const int d = d0 + (lane & 31);
+      f32x4 r;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = *reinterpret_cast<const float*>(tile + row0 * ROW + offset(8 * step + 4 * half + j, d >> 2) + 4 * (d & 3));
+      return r;
+    } else {
+      // 16 lanes read four rows x 32 bytes (lane i: row i / 4, 8-byte piece i % 4) and receive column lane % 16 of those four rows
+      const int i = lane & 15, piece = i & 3, chunk = (d0 >> 3) + 2 * ((lane >> 4) & 1) + (piece >> 1);
+      union {
+        s16x4 q[2];
+        bf16x8 f;
+      } u;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {  // 16 step leaves the swizzle of a row as it is
+        const char* p = tile + (row0 + 16 * step) * ROW + offset(4 * half + 8 * s + (i >> 2), chunk) + 8 * (piece & 1);
+        u.q[s] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+      }
+      return u.f;
+    }
+  }
+};
+
+struct MhaArgs {
+  const void *q, *k, *v, *out, *dout;
+  long qs[3], ks[3], vs[3], os[3], dos[3];  // element strides: batch, token, head
+  const unsigned char* mask;
+  long mask_sb, mask_sl;
+  const float* lse;
+  float* delta;
+  int B, Lq, Lk, H, Hkv, G, D, causal;
+  int rows;         // Lq * G
+  float scale, c;   // c = |scale| * log2(e), never 0 (a scale of 0: 1e-30)
+  int nblk, nsplit, per_split;  // blocks of rows (keys) per key head, splits of the other axis and its length of one split
+};
+
+struct Where {
+  int blk, split, hk;
+  long b;
+};
+// Workgroups go round the 8 XCDs in turn; each XCD gets a contiguous range of the work, so that the blocks that read one key head share an L2.
+__device__ __forceinline__ Where where(const MhaArgs& a) {
+  const unsigned n = gridDim.x, per = n / 8, rest = n % 8, x = blockIdx.x % 8, y = blockIdx.x / 8;
+  unsigned id = x * per + min(x, rest) + y;
+  Where w;
+  w.blk = id % a.nblk;
+  id /= a.nblk;
+  w.split = id % a.nsplit;
+  id /= a.nsplit;
+  w.hk = id % a.Hkv;
+  w.b = id / a.Hkv;
+  return w;
+}
+
+// element offset of row r (= query * G + head of the group) of a tensor with these token / head strides
+__device__ __forceinline__ long row_offset(int r, int G, long sl, long sh) {
+  if (G == 1) return r * sl;
+  const int i = (unsigned)r / (unsigned)G;
+  return i * sl + (r - i * G) * sh;
+}
+
+// B operand of a row product: this lane's row, all steps of the contraction
+template <typename T, int DK>
+struct RowFrags {
+  typename Elem<T>::Frag f[DK / Elem<T>::STEP];
+  __device__ __forceinline__ void load(const T* row, bool on, int D, int lane) {
+#pragma unroll
+    for (int s = 0; s < DK / Elem<T>::STEP; ++s) {
+      const uint4 u = on ? load_chunk<T>(row, 2 * s + (lane >> 5), D, 1) : make_uint4(0, 0, 0, 0);
+      memcpy(&f[s], &u, 16);
+    }
+  }
+  __device__ __forceinline__ void negate() {
+#pragma unroll
+    for (int s = 0; s < DK / Elem<T>::STEP; ++s) f[s] = -f[s];
+  }
+};
+
+// ROWS consecutive rows of a tensor on their way into an LDS tile, held in registers by NT threads.  Buffer loads: the tile's first row is a
+// scalar base, a thread's places in a tile are offsets that do not change, and a place that does not exist is an offset out of range,
+// for which the load returns zeros.  LINEAR: rows are one stride apart (keys), else at places(r) (queries of several heads).
+template <typename T, int W, int ROWS, int NT, bool LINEAR>
+struct Stage {
+  static constexpr int NC = Tile<T, W>::NC, N = (ROWS * NC + NT - 1) / NT, STEP = NT / NC;
+  static_assert(NT % NC == 0 && (N == 1 || ROWS * NC % NT == 0), "every thread holds the same chunk of N rows");
+  static constexpr int NOWHERE = 0x7FFFFFF0;
+  typedef int i32x4 __attribute__((ext_vector_type(4)));
+  i32x4 r[N];
+  int off[LINEAR ? 1 : N];  // byte offsets from the tile's first row
+  int hop;                  // LINEAR: bytes between a thread's rows
+
+  __device__ __forceinline__ static int row(int n) { return n * STEP + (int)threadIdx.x / NC; }
+  __device__ __forceinline__ static int chunk() { return (int)threadIdx.x % NC; }
+
+  __device__ __forceinline__ void linear(long stride, int D) {
+    static_assert(LINEAR, "");
+    off[0] = chunk() * Elem<T>::PER_CHUNK < D && row(0) < ROWS ? (int)(row(0) * stride * (long)sizeof(T)) + chunk() * 16 : NOWHERE;
+    hop = (int)(STEP * stride * (long)sizeof(T));
+  }
+  template <typename Offset>
+  __device__ __forceinline__ void places(Offset offset, int D) {
+    static_assert(!LINEAR, "");
+    const bool on = chunk() * Elem<T>::PER_CHUNK < D && row(0) < ROWS;
+#pragma unroll
+    for (int n = 0; n < N; ++n) off[n] = on ? (int)(offset(row(n)) * (long)sizeof(T)) + chunk() * 16 : NOWHERE;
+  }
+  // rows [from, to) of the tile exist
+  __device__ __forceinline__ void load(const T* first, int from, int to) {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)first, 0, NOWHERE, 0x00020000);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      r[n] = __builtin_amdgcn_raw_buffer_load_b128(rs, (LINEAR || row(n) >= from) && row(n) < to ? off[LINEAR ? 0 : n] : NOWHERE, LINEAR ? n * hop : 0, 0);
+  }
+  __device__ __forceinline__ void put(char* tile) const {
+    if (row(0) >= ROWS) return;
+#pragma unroll
+    for (int n = 0; n < N; ++n) *reinterpret_cast<i32x4*>(tile + Tile<T, W>::offset(row(n), chunk())) = r[n];
+  }
+  // zeros in the rows whose bit is not set
+  template <int NW>
+  __device__ __forceinline__ void hide(const unsigned long (&word)[NW]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int i = row(n);
+      unsigned long w = word[0];
+#pragma unroll
+      for (int x = 1; x < NW; ++x) w = i >= 64 * x ? word[x] : w;
+      if (!(w >> (i & 63) & 1)) r[n] = i32x4{0, 0, 0, 0};
+    }
+  }
+};
+
+// KT keys from k0 on: bit j of word[j / 64] = key k0 + j is below `kend` and not masked.  The bytes are asked for a tile ahead.
+template <int KT>
+struct KeyBits {
+  static constexpr int NW = (KT + 63) / 64;
+  int hidden[NW];
+  unsigned long word[NW];
+  __device__ __forceinline__ void load(const unsigned char* mask, long stride, int k0, int kend, int lane) {
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      const int j = k0 + 64 * x + lane;
+      hidden[x] = j >= kend || (mask && mask[j * stride]);
+    }
+  }
+  __device__ __forceinline__ void settle() {
+#pragma unroll
+    for (int x = 0; x < NW; ++x) word[x] = __ballot(!hidden[x]);
+  }
+  __device__ __forceinline__ bool full() const {
+    bool f = true;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) f = f && word[x] == (KT % 64 && x == NW - 1 ? (1ul << KT % 64) - 1 : ~0ul);
+    return f;
+  }
+  __device__ __forceinline__ unsigned of(int at) const { return (unsigned)(word[at / 64] >> (at & 63)); }  // 32 keys from `at` on
+};
+
+// the D elements of one row held as accumulators of a transposed product (lane = row, registers = dimensions), times f, to dst
+template <typename T, int ND>
+__device__ __forceinline__ void store_row(T* dst, const f32x16 (&o)[ND], float f, int D, int lane) {
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d = 32 * dt + 8 * q + 4 * (lane >> 5);
+      if (d >= D) continue;
+      if constexpr (sizeof(T) == 2)
+        *reinterpret_cast<uint2*>(dst + d) = tatt_pack_bf16x4(o[dt][4 * q] * f, o[dt][4 * q + 1] * f, o[dt][4 * q + 2] * f, o[dt][4 * q + 3] * f);
+      else
+        *reinterpret_cast<float4*>(dst + d) = make_float4(o[dt][4 * q] * f, o[dt][4 * q + 1] * f, o[dt][4 * q + 2] * f, o[dt][4 * q + 3] * f);
+    }
+}
+
+__device__ __forceinline__ float half_max(float x) { return fmaxf(x, __shfl_xor(x, 32, 64)); }
+__device__ __forceinline__ float half_sum(float x) { return x + __shfl_xor(x, 32, 64); }
+// tile row that accumulator register i of a lane half stands for (+ 4 half)
+__device__ __forceinline__ constexpr int acc_row(int i) { return 8 * (i / 4) + i % 4; }
+
+__device__ __forceinline__ void clear(f32x16& o) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) o[i] = 0.f;
+}
+template <int N>
+__device__ __forceinline__ void clear(f32x16 (&o)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) clear(o[n]);
+}
+
+// bits 0 .. n (n < 0: none, n >= 31: all)
+__device__ __forceinline__ unsigned bits_to(int n) { return n < 0 ? 0u : n >= 31 ? ~0u : (2u << n) - 1u; }
+
+// ---- launch plans ---------------------------------------------------------------------------------------------------------------------
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int FILL = 512;  // workgroups that fill the 256 CUs twice
+
+struct Plan {
+  int wide, nblk, nsplit, per_split;  // wide: waves side by side along the output axis; else along the summed one
+};
+// blocks of 128 along the output axis (32 if it has no more than 32), and the summed axis split while the chip is not full, no finer than 512
+inline Plan plan(long problems, int outer, int inner) {
+  Plan p;
+  p.wide = outer > 32;
+  p.nblk = cdiv(outer, p.wide ? 128 : 32);
+  const long blocks = problems * p.nblk;
+  long n = blocks >= FILL ? 1 : (2 * FILL + blocks - 1) / blocks;
+  if (n > inner / 512) n = inner / 512;
+  if (n < 1) n = 1;
+  p.per_split = cdiv(cdiv(inner, n), 128) * 128;
+  p.nsplit = cdiv(inner, p.per_split);
+  return p;
+}
+
+inline bool sane(int B, int Lq, int Lk, int H, int Hkv, int D) { return B > 0 && Lq > 0 && Lk > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && D > 0; }
+
+// 16-byte rows, and a tile of 128 of them within the 31-bit offsets of a buffer load
+inline bool reachable(const void* p, const long* s, int size) {
+  for (int i = 0; i < 3; ++i)
+    if (s[i] < 0 || s[i] * size % 16) return false;
+  return ((uintptr_t)p & 15) == 0 && (s[1] + s[2]) * size < (1L << 31) / 130;
+}
+
+inline int fill(MhaArgs& a, const char* who, const void* q, const void* k, const void* v, const void* out, const void* dout, const long* strides,
+                const unsigned char* mask, const long* mask_strides, int B, int Lq, int Lk, int H, int Hkv, int D, float scale, int causal, int dtype,
+                const float* workspace) {
+  TATT_CHECK_ARG(q && k && v && out && strides && B > 0 && Lq > 0 && Lk > 0 && H > 0 && Hkv > 0, "%s: bad arguments", who);
+  TATT_CHECK_ARG(!mask || mask_strides, "%s: a key mask needs its strides", who);
+  TATT_CHECK_ARG(H % Hkv == 0, "%s: %d query heads are no multiple of %d key heads", who, H, Hkv);
+  TATT_CHECK_ARG(D > 0 && D <= 128, "%s: built for heads of 1 to 128, got %d", who, D);
+  TATT_CHECK_ARG(dtype == TATT_T_F32 || dtype == TATT_T_BF16, "%s: unknown element type %d", who, dtype);
+  TATT_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "%s: the workspace is not 16-byte aligned", who);
+  TATT_CHECK_ARG((long)B * H * Lq < (1L << 30) && (long)B * Hkv * Lk < (1L << 30), "%s: 2^30 rows or more", who);
+  a.q = q, a.k = k, a.v = v, a.out = out, a.dout = dout, a.mask = mask;
+  a.mask_sb = mask ? mask_strides[0] : 0, a.mask_sl = mask ? mask_strides[1] : 0;
+  for (int i = 0; i < 3; ++i) a.qs[i] = strides[i], a.ks[i] = strides[3 + i], a.vs[i] = strides[6 + i];
+  if (dout)
+    for (int i = 0; i < 3; ++i) a.os[i] = strides[9 + i], a.dos[i] = strides[12 + i];
+  const int size = dtype == TATT_T_BF16 ? 2 : 4;
+  TATT_CHECK_ARG(D * size % 16 == 0 && reachable(q, a.qs, size) && reachable(k, a.ks, size) && reachable(v, a.vs, size) && reachable(out, a.os, size) &&
+                     (!dout || reachable(dout, a.dos, size)),
+                 "%s: rows of whole 16 bytes at 16-byte aligned places (and strides of at most 2^24 bytes) expected", who);
+  a.B = B, a.Lq = Lq, a.Lk = Lk, a.H = H, a.Hkv = Hkv, a.G = H / Hkv, a.D = D, a.causal = causal;
+  a.rows = Lq * a.G;
+  a.scale = scale;
+  a.c = scale == 0.f ? 1e-30f : fabsf(scale) * LOG2E;
+  return TATT_OK;
+}
+
+// the grid of one workgroup of `threads` per block, key head and split; more LDS than 64 KB has to be asked for
+template <typename K>
+int prepare_launch(const MhaArgs& a, K kernel, int threads, size_t bytes) {
+  TATT_CHECK_ARG((long)a.B * a.Hkv * a.nblk * a.nsplit * threads < (1L << 32), "tatt_mha: %d x %d x %d x %d workgroups exceed the grid", a.B, a.Hkv, a.nblk, a.nsplit);
+  if (bytes > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != hipSuccess) {
+    (void)hipGetLastError();
+    tatt_set_error("tatt_mha: %zu bytes of LDS refused", bytes);
+    return TATT_ERR_LAUNCH;
+  }
+  return TATT_OK;
+}
+
+template <typename T, int DK>
+struct Shape {
+  static constexpr int W = row_width(DK), ROW = Tile<T, W>::ROW;
+  static constexpr int WK = ROW > 256 ? 2 : 4;  // waves along the summed axis: two tiles of 32 WK rows within 64 KB
+};
+
+}  // namespace
+
+// body with DK bound to the head width rounded up to what the kernels are built for
+#define TATT_DISPATCH_WIDTH(D, ...)             \
+  do {                                          \
+    if ((D) <= 16) {                            \
+      constexpr int DK = 16;                    \
+      __VA_ARGS__                               \
+    } else if ((D) <= 32) {                     \
+      constexpr int DK = 32;                    \
+      __VA_ARGS__                               \
+    } else if ((D) <= 64) {                     \
+      constexpr int DK = 64;                    \
+      __VA_ARGS__                               \
+    } else if ((D) <= 96) {                     \
+      constexpr int DK = 96;                    \
+      __VA_ARGS__                               \
+    } else {                                    \
+      constexpr int DK = 128;                   \
+      __VA_ARGS__                               \
+    }                                           \
+  } while (0)

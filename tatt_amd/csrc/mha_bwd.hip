@@ -1,0 +1,373 @@
+// Attention of any lengths, head counts and head widths up to 128, backward (mha.h has the mathematics and the layouts).
+// The probabilities are recomputed from lse, once in the kernel whose rows are queries (dQ, and delta on the way) and once in the one whose rows
+// are keys (dK, dV): seven products instead of the five that atomics into dQ would need, and sums in a fixed order.
+#include "mha.h"
+
+namespace {
+
+// dQ and delta.  WQ waves of 32 rows; registers hold Q and dO, LDS tiles of 32 SUB keys K and V.
+template <typename T, int DK, int WQ, int SUB>
+__global__ __launch_bounds__(64 * WQ, dq_waves<T>(DK)) void mha_dq_kernel(MhaArgs a, T* __restrict__ dq, float* __restrict__ part) {
+  constexpr int NT = 64 * WQ, W = row_width(DK), ND = (DK + 31) / 32, KT = 32 * SUB, TILE = KT * Tile<T, W>::ROW;
+  constexpr int NS = DK / Elem<T>::STEP, TS = 32 / Elem<T>::STEP, NB = 4 * TILE <= 64 * 1024 ? 2 : 1;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int lane = threadIdx.x & 63, wq = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+  const Where w = where(a);
+  const int blk = a.causal ? a.nblk - 1 - w.blk : w.blk;
+  const int row0 = blk * 32 * WQ, row = row0 + 32 * wq + (lane & 31), past = a.Lk - a.Lq;
+  const bool on = row < a.rows;
+  const int safe = min(row, a.rows - 1), query = (unsigned)safe / (unsigned)a.G, h = w.hk * a.G + safe - query * a.G;
+  const int first_query = (row0 + 32 * wq) / a.G, last_query = min(a.rows - 1, row0 + 32 * wq + 31) / a.G;
+  const T* kb = (const T*)a.k + w.b * a.ks[0] + w.hk * a.ks[2];
+  const T* vb = (const T*)a.v + w.b * a.vs[0] + w.hk * a.vs[2];
+  const unsigned char* mb = a.mask ? a.mask + w.b * a.mask_sb : nullptr;
+
+  RowFrags<T, DK> qf, gf;
+  qf.load((const T*)a.q + w.b * a.qs[0] + query * a.qs[1] + h * a.qs[2], on, a.D, lane);
+  gf.load((const T*)a.dout + w.b * a.dos[0] + query * a.dos[1] + h * a.dos[2], on, a.D, lane);
+  if (a.scale < 0.f) qf.negate();
+  float delta = 0.f;
+  {
+    const T* orow = (const T*)a.out + w.b * a.os[0] + query * a.os[1] + h * a.os[2];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const uint4 u = load_chunk<T>(orow, 2 * s + half, a.D, 1);
+      T t[Elem<T>::PER_CHUNK];
+      memcpy(t, &u, 16);
+#pragma unroll
+      for (int e = 0; e < Elem<T>::PER_CHUNK; ++e) delta += to_f32(t[e]) * (float)gf.f[s][e];
+    }
+    delta = half_sum(delta);
+  }
+  const long stat = (w.b * a.H + h) * a.Lq + query;
+  const float lse = on ? a.lse[stat] : INFINITY;
+  const bool empty = lse == INFINITY;
+  if (empty) delta = 0.f;  // whatever dO holds there
+  if (on && half == 0 && w.split == 0) a.delta[stat] = delta;
+
+  const int kbeg = w.split * a.per_split;
+  int kend = min(a.Lk, kbeg + a.per_split);
+  if (a.causal) kend = min(kend, min(a.rows - 1, row0 + 32 * WQ - 1) / a.G + past + 1);
+  f32x16 o[ND];
+  clear(o);
+  Stage<T, W, KT, NT, true> ks, vs;
+  KeyBits<KT> next, now;
+  ks.linear(a.ks[1], a.D);
+  vs.linear(a.vs[1], a.D);
+  auto fetch = [&](int k0) {
+    ks.load(kb + k0 * a.ks[1], 0, kend - k0);
+    vs.load(vb + k0 * a.vs[1], 0, kend - k0);
+    next.load(mb, a.mask_sl, k0, kend, lane);
+  };
+  auto put = [&](char* to) {
+    next.settle();
+    if (mb && !next.full()) {
+      ks.hide(next.word);
+      vs.hide(next.word);
+    }
+    ks.put(to);
+    vs.put(to + TILE);
+    now = next;
+  };
+  auto step = [&](const char* kt, int k0, auto all) {
+    constexpr bool ALL = decltype(all)::value;
+    const char* vt = kt + TILE;
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+      f32x16 sc, dp;
+      clear(sc);
+      clear(dp);
+#pragma unroll
+      for (int t = 0; t < NS; ++t) sc = mma(Tile<T, W>::rows(kt, 32 * s, t, lane), qf.f[t], sc);
+#pragma unroll
+      for (int t = 0; t < NS; ++t) dp = mma(Tile<T, W>::rows(vt, 32 * s, t, lane), gf.f[t], dp);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], a.c, -lse)) * (dp[i] - delta);
+      if constexpr (!ALL) {
+        const unsigned see = (now.of(32 * s) & (a.causal ? bits_to(query + past - k0 - 32 * s) : ~0u)) >> (4 * half);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[i] = see >> acc_row(i) & 1 ? sc[i] : 0.f;
+      }
+#pragma unroll
+      for (int t = 0; t < TS; ++t) {
+        const auto p = pack_step<T>(sc, t);
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) o[dt] = mma(Tile<T, W>::transposed(kt, 32 * s, t, 32 * dt, lane), p, o[dt]);
+      }
+    }
+  };
+  int at = 0;
+  if (kbeg < kend) {
+    fetch(kbeg);
+    put(lds);
+    if (NB == 2 && kbeg + KT < kend) fetch(kbeg + KT);
+    __syncthreads();
+  }
+  for (int k0 = kbeg; k0 < kend; k0 += KT) {
+    if (NB == 1 && k0 + KT < kend) fetch(k0 + KT);
+    unsigned any = 0;
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) any |= now.of(32 * s);
+    if (any && !(a.causal && last_query + past < k0)) {
+      if (now.full() && !(a.causal && first_query + past < k0 + KT - 1))
+        step(lds + at, k0, std::true_type());
+      else
+        step(lds + at, k0, std::false_type());
+    }
+    if (k0 + KT < kend) {
+      if (NB == 1) __syncthreads();
+      if (NB == 2) at = 2 * TILE - at;
+      put(lds + at);
+      if (NB == 2 && k0 + 2 * KT < kend) fetch(k0 + 2 * KT);
+      __syncthreads();
+    }
+  }
+  if (!on) return;
+  if (empty) clear(o);
+  const long r = (w.b * a.Lq + query) * a.H + h;
+  if (part)
+    store_row<float, ND>(part + (w.split * (long)a.B * a.H * a.Lq + r) * a.D, o, a.scale, a.D, lane);
+  else
+    store_row<T, ND>(dq + r * a.D, o, a.scale, a.D, lane);
+}
+
+// dK and dV.  WN waves along the keys (32 each) x WR along the rows; LDS holds tiles of 32 WR rows of Q and dO, and their lse and delta.
+template <typename T, int DK, int WN, int WR>
+__global__ __launch_bounds__(64 * WN * WR, dkv_waves<T>(DK)) void mha_dkv_kernel(MhaArgs a, T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part) {
+  constexpr int NT = 64 * WN * WR, W = row_width(DK), ND = (DK + 31) / 32, RT = 32 * WR, TILE = RT * Tile<T, W>::ROW, BUF = 2 * TILE + 2 * RT * 4;
+  constexpr int NS = DK / Elem<T>::STEP, TS = 32 / Elem<T>::STEP, NB = 4 * TILE <= 64 * 1024 ? 2 : 1;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wr = wave / WN, half = lane >> 5;
+  const Where w = where(a);
+  const int key0 = w.blk * 32 * WN, key = key0 + 32 * wn + (lane & 31), past = a.Lk - a.Lq;
+  const bool on = key < a.Lk && !(a.mask && a.mask[w.b * a.mask_sb + (long)key * a.mask_sl]);
+  const long key_safe = min(key, a.Lk - 1);
+  RowFrags<T, DK> kf, vf;
+  kf.load((const T*)a.k + w.b * a.ks[0] + key_safe * a.ks[1] + w.hk * a.ks[2], on, a.D, lane);
+  vf.load((const T*)a.v + w.b * a.vs[0] + key_safe * a.vs[1] + w.hk * a.vs[2], on, a.D, lane);
+  if (a.scale < 0.f) kf.negate();
+  const T* qb = (const T*)a.q + w.b * a.qs[0] + w.hk * a.G * a.qs[2];
+  const T* gb = (const T*)a.dout + w.b * a.dos[0] + w.hk * a.G * a.dos[2];
+  const float* lse = a.lse + (w.b * a.H + w.hk * a.G) * a.Lq;
+  const float* delta = a.delta + (w.b * a.H + w.hk * a.G) * a.Lq;
+
+  // causal: this key is seen from row G (key - past) on; rows before the first query that sees anything hold what they like
+  const int first_row = a.causal ? a.G * max(0, key - past) : 0;
+  const int all_rows = a.causal ? a.G * max(0, key0 + 32 * wn + 31 - past) : 0;  // from here on every key of the wave is seen
+  const int none_rows = a.causal ? a.G * max(0, key0 + 32 * wn - past) : 0;      // below this none is
+  const int empty_rows = a.causal ? a.G * max(0, -past) : 0;
+  const bool whole = __all(on);
+  int rbeg = w.split * a.per_split;
+  const int rend = min(a.rows, rbeg + a.per_split);
+  if (a.causal) rbeg = max(rbeg, a.G * max(0, key0 - past) / RT * RT);
+  f32x16 ok[ND], ov[ND];
+  clear(ok);
+  clear(ov);
+  const bool any = __syncthreads_or(on);  // nothing to do where every key of the block is masked
+
+  Stage<T, W, RT, NT, false> qs, gs;
+  float l0 = 0.f, d0 = 0.f;
+  const bool steady = 32 % a.G == 0;  // a tile's rows are the same (query, head) places from its first query on
+  auto places = [&](int r0) {
+    const int i0 = r0 / a.G;
+    qs.places([&](int r) { return row_offset(r0 + r, a.G, a.qs[1], a.qs[2]) - i0 * a.qs[1]; }, a.D);
+    gs.places([&](int r) { return row_offset(r0 + r, a.G, a.dos[1], a.dos[2]) - i0 * a.dos[1]; }, a.D);
+  };
+  auto fetch = [&](int r0) {
+    if (!steady) places(r0);
+    const int i0 = r0 / a.G;
+    qs.load(qb + i0 * a.qs[1], empty_rows - r0, rend - r0);
+    gs.load(gb + i0 * a.dos[1], empty_rows - r0, rend - r0);
+    if (threadIdx.x < RT) {
+      const int r = r0 + threadIdx.x;
+      const bool there = r < rend && r >= empty_rows;
+      const int i = (unsigned)min(r, a.rows - 1) / (unsigned)a.G;
+      const long at = (long)(min(r, a.rows - 1) - i * a.G) * a.Lq + i;
+      l0 = there ? lse[at] : INFINITY;
+      d0 = there ? delta[at] : 0.f;
+    }
+  };
+  auto put = [&](char* to) {
+    qs.put(to);
+    gs.put(to + TILE);
+    float* ls = reinterpret_cast<float*>(to + 2 * TILE);
+    if (threadIdx.x < RT) ls[threadIdx.x] = l0, ls[RT + threadIdx.x] = d0;
+  };
+  auto step = [&](const char* qt, int r0, auto all) {
+    constexpr bool ALL = decltype(all)::value;
+    const char* gt = qt + TILE;
+    const float* ls = reinterpret_cast<const float*>(qt + 2 * TILE);
+    const int at = 32 * wr;
+    f32x16 sc, dp;
+    clear(sc);
+    clear(dp);
+#pragma unroll
+    for (int t = 0; t < NS; ++t) sc = mma(Tile<T, W>::rows(qt, at, t, lane), kf.f[t], sc);
+#pragma unroll
+    for (int t = 0; t < NS; ++t) dp = mma(Tile<T, W>::rows(gt, at, t, lane), vf.f[t], dp);
+    const int hidden = first_row - r0 - at - 4 * half;  // accumulator rows below this are causally hidden
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 lq = *reinterpret_cast<const f32x4*>(ls + at + 8 * q + 4 * half), dq = *reinterpret_cast<const f32x4*>(ls + RT + at + 8 * q + 4 * half);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 4 * q + e;
+        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], a.c, -lq[e]));
+        if constexpr (!ALL) p = on && acc_row(i) >= hidden ? p : 0.f;
+        sc[i] = p;
+        dp[i] = p * (dp[i] - dq[e]);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < TS; ++t) {
+      const auto p = pack_step<T>(sc, t);
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) ov[dt] = mma(Tile<T, W>::transposed(gt, at, t, 32 * dt, lane), p, ov[dt]);
+    }
+#pragma unroll
+    for (int t = 0; t < TS; ++t) {
+      const auto p = pack_step<T>(dp, t);
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) ok[dt] = mma(Tile<T, W>::transposed(qt, at, t, 32 * dt, lane), p, ok[dt]);
+    }
+  };
+  if (any && rbeg < rend) {
+    int at = 0;
+    if (steady) places(0);
+    fetch(rbeg);
+    put(lds);
+    if (NB == 2 && rbeg + RT < rend) fetch(rbeg + RT);
+    __syncthreads();
+    for (int r0 = rbeg; r0 < rend; r0 += RT) {
+      if (NB == 1 && r0 + RT < rend) fetch(r0 + RT);
+      const int mine = r0 + 32 * wr;
+      if (mine + 31 >= none_rows) {
+        if (whole && mine >= all_rows)
+          step(lds + at, r0, std::true_type());
+        else
+          step(lds + at, r0, std::false_type());
+      }
+      if (r0 + RT < rend) {
+        if (NB == 1) __syncthreads();
+        if (NB == 2) at = BUF - at;
+        put(lds + at);
+        if (NB == 2 && r0 + 2 * RT < rend) fetch(r0 + 2 * RT);
+        __syncthreads();
+      }
+    }
+  }
+  if constexpr (WR > 1) {  // sum the waves along the rows in LDS, one of the two gradients at a time: [WN][32 keys][W + 4] added to in wave order
+    float* os = reinterpret_cast<float*>(lds) + (wn * 32 + (lane & 31)) * (W + 4);
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+      for (int x = WR - 1; x >= 0; --x) {
+        __syncthreads();
+        if (wr != x) continue;
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            f32x16& o = which ? ok[dt] : ov[dt];
+            float4* p = reinterpret_cast<float4*>(os + 32 * dt + 8 * q + 4 * half);
+            float4 s = x == WR - 1 ? make_float4(0, 0, 0, 0) : *p;
+            s.x += o[4 * q], s.y += o[4 * q + 1], s.z += o[4 * q + 2], s.w += o[4 * q + 3];
+            if (x)
+              *p = s;
+            else
+              o[4 * q] = s.x, o[4 * q + 1] = s.y, o[4 * q + 2] = s.z, o[4 * q + 3] = s.w;
+          }
+      }
+    if (wr) return;
+  }
+  if (key >= a.Lk) return;
+  const long r = (w.b * a.Lk + key) * a.Hkv + w.hk;
+  if (part) {
+    const long R = (long)a.B * a.Lk * a.Hkv;
+    store_row<float, ND>(part + ((w.split * 2L) * R + r) * a.D, ok, a.scale, a.D, lane);
+    store_row<float, ND>(part + ((w.split * 2L + 1) * R + r) * a.D, ov, 1.f, a.D, lane);
+  } else {
+    store_row<T, ND>(dk + r * a.D, ok, a.scale, a.D, lane);
+    store_row<T, ND>(dv + r * a.D, ov, 1.f, a.D, lane);
+  }
+}
+
+// y[i] = sum over splits of part[split][i] in split order; two tensors of n values each where y2
+template <typename T>
+__global__ __launch_bounds__(256) void mha_sum_kernel(const float* __restrict__ part, int nsplit, long n, T* __restrict__ y, T* __restrict__ y2) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x, all = y2 ? 2 * n : n;
+  if (i >= all) return;
+  float s = 0.f;
+  for (int k = 0; k < nsplit; ++k) s += part[k * all + i];
+  (i < n ? y : y2)[i < n ? i : i - n] = from_f32<T>(s);
+}
+
+Plan plan_dq(int B, int Lq, int Lk, int H, int Hkv) { return plan((long)B * Hkv, Lq * (H / Hkv), Lk); }
+Plan plan_dkv(int B, int Lq, int Lk, int H, int Hkv) { return plan((long)B * Hkv, Lk, Lq * (H / Hkv)); }
+
+template <typename T, int DK, int WN, int WR>
+int launch_dkv(const MhaArgs& a, T* dk, T* dv, float* part, hipStream_t st) {
+  using S = Shape<T, DK>;
+  const size_t tiles = 2 * 32 * WR * S::ROW, buf = tiles + 2 * 32 * WR * 4, join = WR > 1 ? (size_t)WN * 32 * (S::W + 4) * 4 : 0;
+  size_t lds = 2 * tiles <= 64 * 1024 ? 2 * buf : buf;
+  if (join > lds) lds = join;
+  if (int rc = prepare_launch(a, mha_dkv_kernel<T, DK, WN, WR>, 64 * WN * WR, lds)) return rc;
+  hipLaunchKernelGGL((mha_dkv_kernel<T, DK, WN, WR>), dim3((unsigned)((long)a.B * a.Hkv * a.nblk * a.nsplit)), dim3(64 * WN * WR), lds, st, a, dk, dv, part);
+  TATT_LAUNCH_CHECK("mha_dkv");
+  return TATT_OK;
+}
+
+template <typename T, int DK>
+int run_bwd(MhaArgs& a, T* dq, T* dk, T* dv, float* part, hipStream_t st) {
+  using S = Shape<T, DK>;
+  Plan p = plan_dq(a.B, a.Lq, a.Lk, a.H, a.Hkv);
+  a.nblk = cdiv(a.rows, 128), a.nsplit = p.nsplit, a.per_split = p.per_split;
+  {
+    constexpr int SUB = 2;
+    const size_t tiles = 2 * 32 * SUB * S::ROW, lds = 2 * tiles <= 64 * 1024 ? 2 * tiles : tiles;
+    if (int rc = prepare_launch(a, mha_dq_kernel<T, DK, 4, SUB>, 256, lds)) return rc;
+    hipLaunchKernelGGL((mha_dq_kernel<T, DK, 4, SUB>), dim3((unsigned)((long)a.B * a.Hkv * a.nblk * a.nsplit)), dim3(256), lds, st, a, dq,
+                       a.nsplit > 1 ? part : nullptr);
+    TATT_LAUNCH_CHECK("mha_dq");
+    if (a.nsplit > 1) {
+      const long n = (long)a.B * a.H * a.Lq * a.D;
+      hipLaunchKernelGGL(mha_sum_kernel<T>, dim3(cdiv(n, 256)), dim3(256), 0, st, part, a.nsplit, n, dq, (T*)nullptr);
+      TATT_LAUNCH_CHECK("mha_sum");
+    }
+  }
+  p = plan_dkv(a.B, a.Lq, a.Lk, a.H, a.Hkv);
+  a.nblk = p.nblk, a.nsplit = p.nsplit, a.per_split = p.per_split;
+  float* kv_part = a.nsplit > 1 ? part : nullptr;
+  if (int rc = p.wide ? launch_dkv<T, DK, 4, 1>(a, dk, dv, kv_part, st) : launch_dkv<T, DK, 1, S::WK>(a, dk, dv, kv_part, st)) return rc;
+  if (kv_part) {
+    const long n = (long)a.B * a.Hkv * a.Lk * a.D;
+    hipLaunchKernelGGL(mha_sum_kernel<T>, dim3(cdiv(2 * n, 256)), dim3(256), 0, st, part, a.nsplit, n, dk, dv);
+    TATT_LAUNCH_CHECK("mha_sum");
+  }
+  return TATT_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t tatt_mha_bwd_workspace(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype) {
+  if (!sane(B, Lq, Lk, H, Hkv, D)) return 0;
+  const Plan p = plan_dq(B, Lq, Lk, H, Hkv), q = plan_dkv(B, Lq, Lk, H, Hkv);
+  const size_t a = p.nsplit == 1 ? 0 : (size_t)p.nsplit * B * H * Lq * D, b = q.nsplit == 1 ? 0 : (size_t)q.nsplit * 2 * B * Hkv * Lk * D;
+  return ((size_t)B * H * Lq + 3) / 4 * 4 + (a > b ? a : b);  // delta, then the partial sums of one kernel at a time
+}
+
+int tatt_mha_bwd(const void* q, const void* k, const void* v, const long* strides, const unsigned char* mask, const long* mask_strides,
+                 const void* out, const void* dout, const float* lse, void* dq, void* dk, void* dv, int B, int Lq, int Lk, int H, int Hkv, int D,
+                 float scale, int causal, int dtype, float* workspace, hipStream_t st) {
+  MhaArgs a = {};
+  TATT_CHECK_ARG(out && dout && lse && dq && dk && dv && workspace, "tatt_mha_bwd: bad arguments (workspace: tatt_mha_bwd_workspace floats)");
+  if (int rc = fill(a, "tatt_mha_bwd", q, k, v, out, dout, strides, mask, mask_strides, B, Lq, Lk, H, Hkv, D, scale, causal, dtype, workspace)) return rc;
+  TATT_CHECK_ARG((((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) == 0, "tatt_mha_bwd: dq, dk and dv are 16-byte aligned");
+  a.lse = lse, a.delta = workspace;
+  float* part = workspace + ((size_t)B * H * Lq + 3) / 4 * 4;
+  TATT_DISPATCH_TYPE(dtype, TATT_DISPATCH_WIDTH(D, return (run_bwd<T, DK>(a, (T*)dq, (T*)dk, (T*)dv, part, st)););;);
+  return TATT_OK;
+}
+
+}  // extern "C"

@@ -2,6 +2,7 @@
 // throughout; a bf16 value is widened exactly when it is read and rounded once (nearest even) when it is stored.
 #pragma once
 #include "common.h"
+#include <type_traits>
 
 #define TATT_T_F32 0
 #define TATT_T_BF16 1

@@ -220,22 +220,37 @@ def _attention_args(q, k, v, mask, scale):
     return dtype, (B, Lq, Lk, H, Hk, D), D ** -0.5 if scale is None else float(scale)
 
 
+def _laid_out(t, dtype):
+    """t as the kernels read it: rows of whole 16 bytes at 16-byte borders, a tile of them within 31-bit offsets; a copy, its rows padded with zeros
+    (which add nothing to a product), if t is not."""
+    sb, sl, sh, sd = t.stride()
+    per = 8 if dtype else 4
+    D = t.shape[3]
+    if sd == 1 and D % per == 0 and sb % per == 0 and sl % per == 0 and sh % per == 0 and t.data_ptr() % 16 == 0 and sl + sh <= 1 << 21:
+        return t
+    if D % per:
+        return torch.nn.functional.pad(t, (0, -D % per)).contiguous()
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def attention_forward(q, k, v, key_padding_mask=None, causal=False, scale=None, need_lse=True):
     """-> (out, lse): `attention` without autograd; lse [B, H, Lq] fp32 (None unless need_lse), the base-2
     logarithm of each row's sum of exponentials (+inf where it sees nothing), is what attention_backward recomputes from."""
     dtype, dims, scale = _attention_args(q, k, v, key_padding_mask, scale)
-    B, Lq, Lk, H, _, D = dims
+    B, Lq, Lk, H, Hk, D = dims
     if B == 0 or Lq == 0 or Lk == 0:
         return q.new_zeros(q.shape), q.new_full((B, H, Lq), float("inf"), dtype=torch.float32) if need_lse else None
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    out = torch.empty(B, Lq, H, D, dtype=q.dtype, device=q.device)
+    q, k, v = _laid_out(q, dtype), _laid_out(k, dtype), _laid_out(v, dtype)
+    P = q.shape[3]
+    dims = (B, Lq, Lk, H, Hk, P)
+    out = torch.empty(B, Lq, H, P, dtype=q.dtype, device=q.device)
     lse = torch.empty(B, H, Lq, dtype=torch.float32, device=q.device) if need_lse else None
     n = lib().cdll.tatt_mha_fwd_workspace(*dims, dtype)
     ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
     mask_strides = None if key_padding_mask is None else _L2(*key_padding_mask.stride())
     _call("tatt_mha_fwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), _L9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]),
           _ptr(key_padding_mask), mask_strides, out.data_ptr(), _ptr(lse), *dims, scale, bool(causal), dtype, _ptr(ws))
-    return out, lse
+    return out if P == D else out[..., :D].contiguous(), lse
 
 
 def attention_backward(dout, q, k, v, out, lse, key_padding_mask=None, causal=False, scale=None):
@@ -247,15 +262,17 @@ def attention_backward(dout, q, k, v, out, lse, key_padding_mask=None, causal=Fa
         raise RuntimeError("tatt_amd attention_backward: out and dout have the shape of q, lse is attention_forward's")
     if B == 0 or Lq == 0 or Lk == 0:
         return q.new_zeros(q.shape), k.new_zeros(k.shape), v.new_zeros(v.shape)
-    q, k, v, out, dout = _rows(q), _rows(k), _rows(v), _rows(out), _rows(dout)
-    dq = torch.empty(B, Lq, H, D, dtype=q.dtype, device=q.device)
-    dk, dv = (torch.empty(B, Lk, Hk, D, dtype=q.dtype, device=q.device) for _ in range(2))
+    q, k, v, out, dout = _laid_out(q, dtype), _laid_out(k, dtype), _laid_out(v, dtype), _laid_out(out, dtype), _laid_out(dout, dtype)
+    P = q.shape[3]
+    dims = (B, Lq, Lk, H, Hk, P)
+    dq = torch.empty(B, Lq, H, P, dtype=q.dtype, device=q.device)
+    dk, dv = torch.empty(2, B, Lk, Hk, P, dtype=q.dtype, device=q.device).unbind()
     ws = torch.empty(lib().cdll.tatt_mha_bwd_workspace(*dims, dtype), dtype=torch.float32, device=q.device)
     mask_strides = None if key_padding_mask is None else _L2(*key_padding_mask.stride())
     _call("tatt_mha_bwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(),
           _L15(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *dout.stride()[:3]), _ptr(key_padding_mask), mask_strides,
           out.data_ptr(), dout.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *dims, scale, bool(causal), dtype, ws.data_ptr())
-    return dq, dk, dv
+    return (dq, dk, dv) if P == D else tuple(t[..., :D].contiguous() for t in (dq, dk, dv))
 
 
 class _AttentionFn(torch.autograd.Function):
