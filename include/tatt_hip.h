@@ -386,8 +386,8 @@ int tatt_rotary(const void* q, const long* q_strides, void* q_out, int Hq, const
 
 /* Attention (nn.MultiheadAttention's core at model/transformer_v2.py:476, :819, of any size): q [B][Lq][H][D], k / v [B][Lk][Hkv][D], D <= 128, H a
  * multiple of Hkv (query head h reads key head h / (H / Hkv)); strides = HOST array of (batch, token, head) for q, k, v (9 values; the
- * backward call: and out, dout, 15 values); rows of whole 16 bytes at 16-byte aligned places (pad D with zeros, which add nothing), token and
- * head strides of less than 2^24 bytes.  key_mask (may be NULL): bytes [B][Lk], not 0 = leave the key out, mask_strides (batch, key).  causal: query i
+ * backward call: and out, dout, 15 values); rows of whole 16 bytes at 16-byte aligned places (pad D with zeros, which add nothing), 128 rows
+ * (tokens x heads of a group) within 2^31 bytes.  key_mask (may be NULL): bytes [B][Lk], not 0 = leave the key out, mask_strides (batch, key).  causal: query i
  * sees key j iff j <= i + Lk - Lq.  out contiguous [B][Lq][H][D]; lse [B][H][Lq] = base-2 logarithm of the sum of the
  * exponentials (NULL if no backward call follows).  A row that sees no key gives zeros, lse = +inf, and no gradient.  The backward call recomputes the probabilities from lse; dq, dk, dv contiguous.
  * workspace: tatt_mha_*_workspace floats (0 = may be NULL). */

@@ -294,11 +294,11 @@ inline Plan plan(long problems, int outer, int inner) {
 
 inline bool sane(int B, int Lq, int Lk, int H, int Hkv, int D) { return B > 0 && Lq > 0 && Lk > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && D > 0; }
 
-// 16-byte rows, and a tile of 128 of them within the 31-bit offsets of a buffer load
-inline bool reachable(const void* p, const long* s, int size) {
+// 16-byte rows, and a tile of 128 of them (G heads of 128 / G tokens) within the 31-bit offsets of a buffer load
+inline bool reachable(const void* p, const long* s, int size, int G) {
   for (int i = 0; i < 3; ++i)
-    if (s[i] < 0 || s[i] * size % 16) return false;
-  return ((uintptr_t)p & 15) == 0 && (s[1] + s[2]) * size < (1L << 31) / 130;
+    if (s[i] < 0 || s[i] >= 1L << 40 || s[i] * size % 16) return false;
+  return ((uintptr_t)p & 15) == 0 && ((128 / G + 2) * s[1] + (G - 1) * s[2]) * size < (1L << 31) - 4096;
 }
 
 inline int fill(MhaArgs& a, const char* who, const void* q, const void* k, const void* v, const void* out, const void* dout, const long* strides,
@@ -317,9 +317,9 @@ inline int fill(MhaArgs& a, const char* who, const void* q, const void* k, const
   if (dout)
     for (int i = 0; i < 3; ++i) a.os[i] = strides[9 + i], a.dos[i] = strides[12 + i];
   const int size = dtype == TATT_T_BF16 ? 2 : 4;
-  TATT_CHECK_ARG(D * size % 16 == 0 && reachable(q, a.qs, size) && reachable(k, a.ks, size) && reachable(v, a.vs, size) && reachable(out, a.os, size) &&
-                     (!dout || reachable(dout, a.dos, size)),
-                 "%s: rows of whole 16 bytes at 16-byte aligned places (and strides of at most 2^24 bytes) expected", who);
+  TATT_CHECK_ARG(D * size % 16 == 0 && reachable(q, a.qs, size, H / Hkv) && reachable(k, a.ks, size, 1) && reachable(v, a.vs, size, 1) &&
+                     reachable(out, a.os, size, H / Hkv) && (!dout || reachable(dout, a.dos, size, H / Hkv)),
+                 "%s: rows of whole 16 bytes at 16-byte aligned places expected, 128 of them within 2^31 bytes", who);
   a.B = B, a.Lq = Lq, a.Lk = Lk, a.H = H, a.Hkv = Hkv, a.G = H / Hkv, a.D = D, a.causal = causal;
   a.rows = Lq * a.G;
   a.scale = scale;

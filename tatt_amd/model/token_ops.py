@@ -220,13 +220,13 @@ def _attention_args(q, k, v, mask, scale):
     return dtype, (B, Lq, Lk, H, Hk, D), D ** -0.5 if scale is None else float(scale)
 
 
-def _laid_out(t, dtype):
-    """t as the kernels read it: rows of whole 16 bytes at 16-byte borders, a tile of them within 31-bit offsets; a copy, its rows padded with zeros
-    (which add nothing to a product), if t is not."""
+def _laid_out(t, dtype, group=1):
+    """t as the kernels read it: rows of whole 16 bytes at 16-byte borders, a tile of 128 (of `group` heads) within 31-bit offsets; a copy, its rows
+    padded with zeros (which add nothing to a product), if t is not."""
     sb, sl, sh, sd = t.stride()
     per = 8 if dtype else 4
     D = t.shape[3]
-    if sd == 1 and D % per == 0 and sb % per == 0 and sl % per == 0 and sh % per == 0 and t.data_ptr() % 16 == 0 and sl + sh <= 1 << 21:
+    if sd == 1 and D % per == 0 and sb % per == 0 and sl % per == 0 and sh % per == 0 and t.data_ptr() % 16 == 0 and (128 // group + 2) * sl + (group - 1) * sh <= 1 << 28:
         return t
     if D % per:
         return torch.nn.functional.pad(t, (0, -D % per)).contiguous()
@@ -240,7 +240,7 @@ def attention_forward(q, k, v, key_padding_mask=None, causal=False, scale=None, 
     B, Lq, Lk, H, Hk, D = dims
     if B == 0 or Lq == 0 or Lk == 0:
         return q.new_zeros(q.shape), q.new_full((B, H, Lq), float("inf"), dtype=torch.float32) if need_lse else None
-    q, k, v = _laid_out(q, dtype), _laid_out(k, dtype), _laid_out(v, dtype)
+    q, k, v = _laid_out(q, dtype, H // Hk), _laid_out(k, dtype), _laid_out(v, dtype)
     P = q.shape[3]
     dims = (B, Lq, Lk, H, Hk, P)
     out = torch.empty(B, Lq, H, P, dtype=q.dtype, device=q.device)
@@ -262,7 +262,8 @@ def attention_backward(dout, q, k, v, out, lse, key_padding_mask=None, causal=Fa
         raise RuntimeError("tatt_amd attention_backward: out and dout have the shape of q, lse is attention_forward's")
     if B == 0 or Lq == 0 or Lk == 0:
         return q.new_zeros(q.shape), k.new_zeros(k.shape), v.new_zeros(v.shape)
-    q, k, v, out, dout = _laid_out(q, dtype), _laid_out(k, dtype), _laid_out(v, dtype), _laid_out(out, dtype), _laid_out(dout, dtype)
+    q, out, dout = (_laid_out(t, dtype, H // Hk) for t in (q, out, dout))
+    k, v = _laid_out(k, dtype), _laid_out(v, dtype)
     P = q.shape[3]
     dims = (B, Lq, Lk, H, Hk, P)
     dq = torch.empty(B, Lq, H, P, dtype=q.dtype, device=q.device)

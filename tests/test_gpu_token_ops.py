@@ -533,3 +533,17 @@ def test_operators_captured_and_replayed(dtype):
         torch.cuda.synchronize()
         for (_, _, res), want in zip(graphs, eager):
             assert all(torch.equal(a, c) for a, c in zip(res, want)), round_
+
+
+def test_attention_reads_long_sequences_where_they_lie():
+    """Head-major keys of 20000 tokens (a head stride of 2.5 million elements), and tokens so far apart that a copy is made: the same result."""
+    q = rnd(1, 4, 1, 128, seed=1, dtype=BF16).transpose(1, 2)
+    k, v = (rnd(1, 2, 20000, 128, seed=s, dtype=BF16).transpose(1, 2) for s in (2, 3))
+    assert T._laid_out(k, 1).data_ptr() == k.data_ptr() and T._laid_out(q, 1, 2).data_ptr() == q.data_ptr()
+    want, lse = T.attention_forward(q, k.contiguous(), v.contiguous())
+    got = T.attention_forward(q, k, v)
+    assert torch.equal(got[0], want) and torch.equal(got[1], lse)
+    far = torch.empty(40 << 22, dtype=BF16, device="cuda").as_strided((1, 40, 2, 128), (40 << 22, 1 << 22, 128, 1))
+    far.copy_(k[:, :40])
+    assert T._laid_out(far, 1).data_ptr() != far.data_ptr()
+    assert torch.equal(T.attention_forward(q, far, far)[0], T.attention_forward(q, k[:, :40], k[:, :40])[0])

@@ -87,3 +87,12 @@ def test_frequencies():
     f = T.rotary_frequencies((4, 8), base=100.0, device="cpu")
     assert f.dtype == torch.float64
     assert torch.allclose(f, torch.tensor([1.0, 0.1, 1.0, 100 ** -0.25, 0.1, 100 ** -0.75], dtype=torch.float64), rtol=1e-15, atol=0)
+
+
+@pytest.mark.parametrize("call,n", [(fwd, 9), (bwd, 15)])
+@pytest.mark.parametrize("kw", [{"D": 6}, {"q": P + 8}, {"k": P + 4}, {"strides": 2}, {"strides": 1 << 25}])
+def test_attention_entry_points_refuse_rows_they_cannot_read(call, n, kw):
+    if "strides" in kw:
+        kw = {"strides": (ctypes.c_long * n)(*[kw["strides"]] * n)}
+    with pytest.raises(RuntimeError, match="16-byte aligned places"):
+        call(**kw)
