@@ -21,6 +21,18 @@
 #pragma once
 #include "token_types.h"
 
+#ifndef FW
+#define FW 2
+#endif
+#ifndef DQ
+#define DQ 2
+#endif
+#ifndef DKV128
+#define DKV128 1
+#endif
+#ifndef DKV
+#define DKV 2
+#endif
 namespace {
 
 __device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
@@ -47,11 +59,11 @@ __device__ __forceinline__ typename Elem<T>::Frag pack_step(const f32x16& c, int
 // waves a SIMD that the registers are shared out for.  Two (256 registers each) unless what a wave has to hold -- the fragments of its rows, the
 // sums, a tile on its way -- would spill: then one, the sums in the other half of the register file.
 template <typename T>
-constexpr int fwd_waves(int DK) { return sizeof(T) == 4 && DK > 64 ? 1 : 2; }
+constexpr int fwd_waves(int DK) { return sizeof(T) == 4 && DK > 64 ? 1 : DK <= 64 ? FW : 2; }
 template <typename T>
-constexpr int dq_waves(int DK) { return sizeof(T) == 4 && DK >= 64 ? 1 : 2; }
+constexpr int dq_waves(int DK) { return sizeof(T) == 4 && DK >= 64 ? 1 : DK <= 64 ? DQ : 2; }
 template <typename T>
-constexpr int dkv_waves(int DK) { return DK > 64 || (sizeof(T) == 4 && DK == 64) ? 1 : 2; }
+constexpr int dkv_waves(int DK) { return (DK > 64 && DKV128) || (sizeof(T) == 4 && DK == 64) ? 1 : DKV; }
 
 // head widths the kernels are built for, and the LDS row that holds one
 constexpr int row_width(int DK) { return DK <= 32 ? 32 : DK <= 64 ? 64 : 128; }
@@ -70,31 +82,48 @@ struct Tile {
   }
   __device__ __forceinline__ static int offset(int r, int chunk) { return r * ROW + ((chunk ^ swizzle(r)) << 4); }
 
-  // A operand of a row product: lane (row = lane % 32, half) holds chunk 2 step + half of its row
-  __device__ __forceinline__ static typename Elem<T>::Frag rows(const char* tile, int row0, int step, int lane) {
-    return *reinterpret_cast<const typename Elem<T>::Frag*>(tile + row0 * ROW + offset(lane & 31, 2 * step + (lane >> 5)));
+  // Where a lane reads: (its base ^ a constant) + a constant, so one register serves every fragment of a kind.
+  struct Lane {
+    int row, col;
+    __device__ __forceinline__ explicit Lane(int lane) {
+      const int half = lane >> 5;
+      row = offset(lane & 31, half);
+      if constexpr (sizeof(T) == 4) {
+        const int d = lane & 31;
+        col = 4 * half * ROW + (((d >> 2) ^ half) << 4) + 4 * (d & 3);
+      } else {  // 16 lanes read four rows x 32 bytes (lane i: row i / 4, 8-byte piece i % 4) and receive column lane % 16 of those four rows
+        const int i = lane & 15, piece = i & 3;
+        col = offset(4 * half + (i >> 2), 2 * ((lane >> 4) & 1) + (piece >> 1)) + 8 * (piece & 1);
+      }
+    }
+    // keeps the compiler from holding each base ^ constant in a register of its own across the loop (and spilling them)
+    __device__ __forceinline__ void afresh() { asm volatile("" : "+v"(row), "+v"(col)); }
+  };
+
+  // A operand of a row product: lane (row = lane % 32, half) holds chunk 2 step + half of its row.  row0 a multiple of 32.
+  __device__ __forceinline__ static typename Elem<T>::Frag rows(const char* tile, int row0, int step, const Lane& at) {
+    return *reinterpret_cast<const typename Elem<T>::Frag*>(tile + row0 * ROW + (at.row ^ (step << 5)));
   }
 
   // A operand of a transposed product: lane (dimension d0 + lane % 32, half) holds the tile rows that accumulator registers of `step` stand for:
   // fp32: row0 + 8 step + 4 half + j;  bf16: row0 + 16 step + 4 half + {0..3, 8..11}.  d0 and row0 multiples of 32.
-  __device__ __forceinline__ static typename Elem<T>::Frag transposed(const char* tile, int row0, int step, int d0, int lane) {
-    const int half = lane >> 5;
+  __device__ __forceinline__ static typename Elem<T>::Frag transposed(const char* tile, int row0, int step, int d0, const Lane& at) {
     if constexpr (sizeof(T) == 4) {
-      const int d = d0 + (lane & 31);
       f32x4 r;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r[j] = *reinterpret_cast<const float*>(tile + row0 * ROW + offset(8 * step + 4 * half + j, d >> 2) + 4 * (d & 3));
+      for (int j = 0; j < 4; ++j) {
+        const int turn = (NC >= 16 ? j << 2 : (j >> 1) << 2) ^ (2 * (step & 1)) ^ (d0 >> 2);  // swizzle of row 8 step + 4 half + j, and the chunk of d0
+        r[j] = *reinterpret_cast<const float*>(tile + (row0 + 8 * step + j) * ROW + (at.col ^ (turn << 4)));
+      }
       return r;
     } else {
-      // 16 lanes read four rows x 32 bytes (lane i: row i / 4, 8-byte piece i % 4) and receive column lane % 16 of those four rows
-      const int i = lane & 15, piece = i & 3, chunk = (d0 >> 3) + 2 * ((lane >> 4) & 1) + (piece >> 1);
       union {
         s16x4 q[2];
         bf16x8 f;
       } u;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {  // 16 step leaves the swizzle of a row as it is
-        const char* p = tile + (row0 + 16 * step) * ROW + offset(4 * half + 8 * s + (i >> 2), chunk) + 8 * (piece & 1);
+      for (int s = 0; s < 2; ++s) {
+        const char* p = tile + (row0 + 16 * step + 8 * s) * ROW + (at.col ^ (((d0 >> 3) ^ (2 * s)) << 4));
         u.q[s] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
       }
       return u.f;
@@ -188,9 +217,14 @@ struct Stage {
   // rows [from, to) of the tile exist
   __device__ __forceinline__ void load(const T* first, int from, int to) {
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)first, 0, NOWHERE, 0x00020000);
+    if (from <= 0 && to >= ROWS) {
 #pragma unroll
-    for (int n = 0; n < N; ++n)
-      r[n] = __builtin_amdgcn_raw_buffer_load_b128(rs, (LINEAR || row(n) >= from) && row(n) < to ? off[LINEAR ? 0 : n] : NOWHERE, LINEAR ? n * hop : 0, 0);
+      for (int n = 0; n < N; ++n) r[n] = __builtin_amdgcn_raw_buffer_load_b128(rs, off[LINEAR ? 0 : n], LINEAR ? n * hop : 0, 0);
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        r[n] = __builtin_amdgcn_raw_buffer_load_b128(rs, row(n) >= from && row(n) < to ? off[LINEAR ? 0 : n] : NOWHERE, LINEAR ? n * hop : 0, 0);
+    }
   }
   __device__ __forceinline__ void put(char* tile) const {
     if (row(0) >= ROWS) return;
@@ -211,22 +245,27 @@ struct Stage {
   }
 };
 
-// KT keys from k0 on: bit j of word[j / 64] = key k0 + j is below `kend` and not masked.  The bytes are asked for a tile ahead.
+// KT keys from k0 on: bit j of word[j / 64] = key k0 + j is below `kend` and not masked.  The mask's bytes are asked for a tile ahead.
 template <int KT>
 struct KeyBits {
   static constexpr int NW = (KT + 63) / 64;
   int hidden[NW];
   unsigned long word[NW];
   __device__ __forceinline__ void load(const unsigned char* mask, long stride, int k0, int kend, int lane) {
+    if (!mask) return;
 #pragma unroll
     for (int x = 0; x < NW; ++x) {
       const int j = k0 + 64 * x + lane;
-      hidden[x] = j >= kend || (mask && mask[j * stride]);
+      hidden[x] = j >= kend || mask[j * stride];
     }
   }
-  __device__ __forceinline__ void settle() {
+  __device__ __forceinline__ void settle(const unsigned char* mask, int k0, int kend) {
 #pragma unroll
-    for (int x = 0; x < NW; ++x) word[x] = __ballot(!hidden[x]);
+    for (int x = 0; x < NW; ++x) {
+      const int n = min(kend - k0, KT) - 64 * x;
+      word[x] = mask ? __ballot(!hidden[x]) : n <= 0 ? 0ul : n >= 64 ? ~0ul : (1ul << n) - 1;
+    }
+    if (mask && KT < 64) word[0] &= (1ul << (KT & 63)) - 1;
   }
   __device__ __forceinline__ bool full() const {
     bool f = true;
@@ -253,8 +292,15 @@ __device__ __forceinline__ void store_row(T* dst, const f32x16 (&o)[ND], float f
     }
 }
 
-__device__ __forceinline__ float half_max(float x) { return fmaxf(x, __shfl_xor(x, 32, 64)); }
-__device__ __forceinline__ float half_sum(float x) { return x + __shfl_xor(x, 32, 64); }
+// over a lane and the one 32 further: v_permlane32_swap_b32, a register exchange (a shuffle through LDS waits some hundred cycles)
+__device__ __forceinline__ float half_max(float x) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
 // tile row that accumulator register i of a lane half stands for (+ 4 half)
 __device__ __forceinline__ constexpr int acc_row(int i) { return 8 * (i / 4) + i % 4; }
 
@@ -342,6 +388,7 @@ int prepare_launch(const MhaArgs& a, K kernel, int threads, size_t bytes) {
 template <typename T, int DK>
 struct Shape {
   static constexpr int W = row_width(DK), ROW = Tile<T, W>::ROW;
+  static constexpr int WKF = ROW > 256 ? 1 : ROW == 256 ? 2 : 4;  // forward: four tiles of 32 WK rows within 64 KB
   static constexpr int WK = ROW > 256 ? 2 : 4;  // waves along the summed axis: two tiles of 32 WK rows within 64 KB
 };
 

@@ -3,6 +3,9 @@
 // are keys (dK, dV): seven products instead of the five that atomics into dQ would need, and sums in a fixed order.
 #include "mha.h"
 
+#ifndef DQSUB
+#define DQSUB 1
+#endif
 namespace {
 
 // dQ and delta.  WQ waves of 32 rows; registers hold Q and dO, LDS tiles of 32 SUB keys K and V.
@@ -59,31 +62,38 @@ __global__ __launch_bounds__(64 * WQ, dq_waves<T>(DK)) void mha_dq_kernel(MhaArg
     vs.load(vb + k0 * a.vs[1], 0, kend - k0);
     next.load(mb, a.mask_sl, k0, kend, lane);
   };
-  auto put = [&](char* to) {
-    next.settle();
-    if (mb && !next.full()) {
-      ks.hide(next.word);
-      vs.hide(next.word);
-    }
+  auto put = [&](char* to, int k0) {
+    next.settle(mb, k0, kend);
+    if (mb && !next.full()) ks.hide(next.word);  // a masked key's dS is replaced, its K would still meet that 0
     ks.put(to);
     vs.put(to + TILE);
     now = next;
   };
-  auto step = [&](const char* kt, int k0, auto all) {
-    constexpr bool ALL = decltype(all)::value;
-    const char* vt = kt + TILE;
+  typename Tile<T, W>::Lane place(lane);
+  int at = 0;
+  if (kbeg < kend) {
+    fetch(kbeg);
+    put(lds, kbeg);
+    if (NB == 2 && kbeg + KT < kend) fetch(kbeg + KT);
+    __syncthreads();
+  }
+  for (int k0 = kbeg; k0 < kend; k0 += KT) {
+    if (NB == 1 && k0 + KT < kend) fetch(k0 + KT);
+    const char *kt = lds + at, *vt = kt + TILE;
+    place.afresh();
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
+      if (now.of(32 * s) == 0 || (a.causal && last_query + past < k0 + 32 * s)) continue;
       f32x16 sc, dp;
       clear(sc);
       clear(dp);
 #pragma unroll
-      for (int t = 0; t < NS; ++t) sc = mma(Tile<T, W>::rows(kt, 32 * s, t, lane), qf.f[t], sc);
+      for (int t = 0; t < NS; ++t) sc = mma(Tile<T, W>::rows(kt, 32 * s, t, place), qf.f[t], sc);
 #pragma unroll
-      for (int t = 0; t < NS; ++t) dp = mma(Tile<T, W>::rows(vt, 32 * s, t, lane), gf.f[t], dp);
+      for (int t = 0; t < NS; ++t) dp = mma(Tile<T, W>::rows(vt, 32 * s, t, place), gf.f[t], dp);
 #pragma unroll
       for (int i = 0; i < 16; ++i) sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], a.c, -lse)) * (dp[i] - delta);
-      if constexpr (!ALL) {
+      if (!now.full() || (a.causal && first_query + past < k0 + 32 * s + 31)) {
         const unsigned see = (now.of(32 * s) & (a.causal ? bits_to(query + past - k0 - 32 * s) : ~0u)) >> (4 * half);
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[i] = see >> acc_row(i) & 1 ? sc[i] : 0.f;
@@ -92,32 +102,13 @@ __global__ __launch_bounds__(64 * WQ, dq_waves<T>(DK)) void mha_dq_kernel(MhaArg
       for (int t = 0; t < TS; ++t) {
         const auto p = pack_step<T>(sc, t);
 #pragma unroll
-        for (int dt = 0; dt < ND; ++dt) o[dt] = mma(Tile<T, W>::transposed(kt, 32 * s, t, 32 * dt, lane), p, o[dt]);
+        for (int dt = 0; dt < ND; ++dt) o[dt] = mma(Tile<T, W>::transposed(kt, 32 * s, t, 32 * dt, place), p, o[dt]);
       }
-    }
-  };
-  int at = 0;
-  if (kbeg < kend) {
-    fetch(kbeg);
-    put(lds);
-    if (NB == 2 && kbeg + KT < kend) fetch(kbeg + KT);
-    __syncthreads();
-  }
-  for (int k0 = kbeg; k0 < kend; k0 += KT) {
-    if (NB == 1 && k0 + KT < kend) fetch(k0 + KT);
-    unsigned any = 0;
-#pragma unroll
-    for (int s = 0; s < SUB; ++s) any |= now.of(32 * s);
-    if (any && !(a.causal && last_query + past < k0)) {
-      if (now.full() && !(a.causal && first_query + past < k0 + KT - 1))
-        step(lds + at, k0, std::true_type());
-      else
-        step(lds + at, k0, std::false_type());
     }
     if (k0 + KT < kend) {
       if (NB == 1) __syncthreads();
       if (NB == 2) at = 2 * TILE - at;
-      put(lds + at);
+      put(lds + at, k0 + KT);
       if (NB == 2 && k0 + 2 * KT < kend) fetch(k0 + 2 * KT);
       __syncthreads();
     }
@@ -193,46 +184,9 @@ __global__ __launch_bounds__(64 * WN * WR, dkv_waves<T>(DK)) void mha_dkv_kernel
     float* ls = reinterpret_cast<float*>(to + 2 * TILE);
     if (threadIdx.x < RT) ls[threadIdx.x] = l0, ls[RT + threadIdx.x] = d0;
   };
-  auto step = [&](const char* qt, int r0, auto all) {
-    constexpr bool ALL = decltype(all)::value;
-    const char* gt = qt + TILE;
-    const float* ls = reinterpret_cast<const float*>(qt + 2 * TILE);
-    const int at = 32 * wr;
-    f32x16 sc, dp;
-    clear(sc);
-    clear(dp);
-#pragma unroll
-    for (int t = 0; t < NS; ++t) sc = mma(Tile<T, W>::rows(qt, at, t, lane), kf.f[t], sc);
-#pragma unroll
-    for (int t = 0; t < NS; ++t) dp = mma(Tile<T, W>::rows(gt, at, t, lane), vf.f[t], dp);
-    const int hidden = first_row - r0 - at - 4 * half;  // accumulator rows below this are causally hidden
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f32x4 lq = *reinterpret_cast<const f32x4*>(ls + at + 8 * q + 4 * half), dq = *reinterpret_cast<const f32x4*>(ls + RT + at + 8 * q + 4 * half);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = 4 * q + e;
-        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], a.c, -lq[e]));
-        if constexpr (!ALL) p = on && acc_row(i) >= hidden ? p : 0.f;
-        sc[i] = p;
-        dp[i] = p * (dp[i] - dq[e]);
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < TS; ++t) {
-      const auto p = pack_step<T>(sc, t);
-#pragma unroll
-      for (int dt = 0; dt < ND; ++dt) ov[dt] = mma(Tile<T, W>::transposed(gt, at, t, 32 * dt, lane), p, ov[dt]);
-    }
-#pragma unroll
-    for (int t = 0; t < TS; ++t) {
-      const auto p = pack_step<T>(dp, t);
-#pragma unroll
-      for (int dt = 0; dt < ND; ++dt) ok[dt] = mma(Tile<T, W>::transposed(qt, at, t, 32 * dt, lane), p, ok[dt]);
-    }
-  };
+  typename Tile<T, W>::Lane place(lane);
   if (any && rbeg < rend) {
-    int at = 0;
+    int buf = 0;
     if (steady) places(0);
     fetch(rbeg);
     put(lds);
@@ -240,17 +194,52 @@ __global__ __launch_bounds__(64 * WN * WR, dkv_waves<T>(DK)) void mha_dkv_kernel
     __syncthreads();
     for (int r0 = rbeg; r0 < rend; r0 += RT) {
       if (NB == 1 && r0 + RT < rend) fetch(r0 + RT);
-      const int mine = r0 + 32 * wr;
-      if (mine + 31 >= none_rows) {
-        if (whole && mine >= all_rows)
-          step(lds + at, r0, std::true_type());
-        else
-          step(lds + at, r0, std::false_type());
+      const int at = 32 * wr;
+      if (r0 + at + 31 >= none_rows) {
+        const char *qt = lds + buf, *gt = qt + TILE;
+        const float* ls = reinterpret_cast<const float*>(qt + 2 * TILE);
+        place.afresh();
+        f32x16 sc, dp;
+        clear(sc);
+        clear(dp);
+#pragma unroll
+        for (int t = 0; t < NS; ++t) sc = mma(Tile<T, W>::rows(qt, at, t, place), kf.f[t], sc);
+#pragma unroll
+        for (int t = 0; t < NS; ++t) dp = mma(Tile<T, W>::rows(gt, at, t, place), vf.f[t], dp);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 lq = *reinterpret_cast<const f32x4*>(ls + at + 8 * q + 4 * half);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[4 * q + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[4 * q + e], a.c, -lq[e]));
+        }
+        if (!whole || r0 + at < all_rows) {
+          const int hidden = first_row - r0 - at - 4 * half;  // accumulator rows below this are causally hidden
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[i] = on && acc_row(i) >= hidden ? sc[i] : 0.f;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 dq = *reinterpret_cast<const f32x4*>(ls + RT + at + 8 * q + 4 * half);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dp[4 * q + e] = sc[4 * q + e] * (dp[4 * q + e] - dq[e]);
+        }
+#pragma unroll
+        for (int t = 0; t < TS; ++t) {
+          const auto p = pack_step<T>(sc, t);
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) ov[dt] = mma(Tile<T, W>::transposed(gt, at, t, 32 * dt, place), p, ov[dt]);
+        }
+#pragma unroll
+        for (int t = 0; t < TS; ++t) {
+          const auto p = pack_step<T>(dp, t);
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) ok[dt] = mma(Tile<T, W>::transposed(qt, at, t, 32 * dt, place), p, ok[dt]);
+        }
       }
       if (r0 + RT < rend) {
         if (NB == 1) __syncthreads();
-        if (NB == 2) at = BUF - at;
-        put(lds + at);
+        if (NB == 2) buf = BUF - buf;
+        put(lds + buf);
         if (NB == 2 && r0 + 2 * RT < rend) fetch(r0 + 2 * RT);
         __syncthreads();
       }
@@ -322,7 +311,7 @@ int run_bwd(MhaArgs& a, T* dq, T* dk, T* dv, float* part, hipStream_t st) {
   Plan p = plan_dq(a.B, a.Lq, a.Lk, a.H, a.Hkv);
   a.nblk = cdiv(a.rows, 128), a.nsplit = p.nsplit, a.per_split = p.per_split;
   {
-    constexpr int SUB = 2;
+    constexpr int SUB = DK > 64 ? DQSUB : 2;
     const size_t tiles = 2 * 32 * SUB * S::ROW, lds = 2 * tiles <= 64 * 1024 ? 2 * tiles : tiles;
     if (int rc = prepare_launch(a, mha_dq_kernel<T, DK, 4, SUB>, 256, lds)) return rc;
     hipLaunchKernelGGL((mha_dq_kernel<T, DK, 4, SUB>), dim3((unsigned)((long)a.B * a.Hkv * a.nblk * a.nsplit)), dim3(256), lds, st, a, dq,

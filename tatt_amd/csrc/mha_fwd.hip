@@ -2,13 +2,22 @@
 // and the layouts).  One pass over the keys with a running maximum and sum; no score leaves the registers.
 #include "mha.h"
 
+#ifndef JT
+#define JT 2
+#endif
+#ifndef SB
+#define SB 2
+#endif
+#ifndef R2MIN
+#define R2MIN 256
+#endif
 namespace {
 
 constexpr float NO_MAX = -1e30f;  // the running maximum before any visible score; finite, so that differences from it are not NaN
 constexpr float LAZY = 8.f;       // the running maximum follows only rises of more than 2^8: P stays below 2^8, and fp32 sums hold that exactly as well
 
-// WQ waves along the rows (32 each) x WK along the keys; SUB tiles of 32 keys for a wave at a time.
-template <typename T, int DK, int WQ, int WK, int SUB>
+// WQ waves along the rows (32 R each) x WK along the keys; tiles of 32 SUB keys for a wave, JOINT of them sharing a look at the maximum.
+template <typename T, int DK, int WQ, int R, int WK, int SUB, int JOINT>
 __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel(MhaArgs a, T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part) {
   constexpr int NT = 64 * WQ * WK, W = row_width(DK), ND = (DK + 31) / 32, KT = 32 * WK * SUB, TILE = KT * Tile<T, W>::ROW;
   constexpr int NS = DK / Elem<T>::STEP, TS = 32 / Elem<T>::STEP, NB = 4 * TILE <= 64 * 1024 ? 2 : 1;
@@ -16,171 +25,204 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wq = wave % WQ, wk = wave / WQ, half = lane >> 5;
   const Where w = where(a);
   const int blk = a.causal ? a.nblk - 1 - w.blk : w.blk;  // causal: the longest blocks first
-  const int row0 = blk * 32 * WQ, row = row0 + 32 * wq + (lane & 31);
+  const int row0 = blk * 32 * WQ * R, wrow0 = row0 + 32 * wq * R, row = wrow0 + (lane & 31);  // and row + 32 r
   const T* kb = (const T*)a.k + w.b * a.ks[0] + w.hk * a.ks[2];
   const T* vb = (const T*)a.v + w.b * a.vs[0] + w.hk * a.vs[2];
   const unsigned char* mb = a.mask ? a.mask + w.b * a.mask_sb : nullptr;
   const int past = a.Lk - a.Lq;
-  const int query = (unsigned)row / (unsigned)a.G;
-  const int first_query = (row0 + 32 * wq) / a.G, last_query = min(a.rows - 1, row0 + 32 * wq + 31) / a.G;
+  const int first_query = wrow0 / a.G, last_query = min(a.rows - 1, wrow0 + 32 * R - 1) / a.G;
 
-  RowFrags<T, DK> qf;
-  qf.load((const T*)a.q + w.b * a.qs[0] + w.hk * a.G * a.qs[2] + row_offset(min(row, a.rows - 1), a.G, a.qs[1], a.qs[2]), row < a.rows, a.D, lane);
-  if (a.scale < 0.f) qf.negate();
+  RowFrags<T, DK> qf[R];
+  int query[R];
+  f32x16 o[R][ND];
+  float m[R], l[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    query[r] = (unsigned)(row + 32 * r) / (unsigned)a.G;
+    qf[r].load((const T*)a.q + w.b * a.qs[0] + w.hk * a.G * a.qs[2] + row_offset(min(row + 32 * r, a.rows - 1), a.G, a.qs[1], a.qs[2]), row + 32 * r < a.rows, a.D, lane);
+    if (a.scale < 0.f) qf[r].negate();
+    clear(o[r]);
+    m[r] = NO_MAX;
+    l[r] = 0.f;
+  }
 
   const int kbeg = w.split * a.per_split;
   int kend = min(a.Lk, kbeg + a.per_split);
-  if (a.causal) kend = min(kend, min(a.rows - 1, row0 + 32 * WQ - 1) / a.G + past + 1);
-
-  f32x16 o[ND];
-  clear(o);
-  float m = NO_MAX, l = 0.f;
+  if (a.causal) kend = min(kend, min(a.rows - 1, row0 + 32 * WQ * R - 1) / a.G + past + 1);
 
   Stage<T, W, KT, NT, true> ks, vs;
   KeyBits<KT> next, now;
   ks.linear(a.ks[1], a.D);
   vs.linear(a.vs[1], a.D);
+  typename Tile<T, W>::Lane place(lane);
   auto fetch = [&](int k0) {
     ks.load(kb + k0 * a.ks[1], 0, kend - k0);
     vs.load(vb + k0 * a.vs[1], 0, kend - k0);
     next.load(mb, a.mask_sl, k0, kend, lane);
   };
-  auto put = [&](char* to) {
-    next.settle();
-    if (mb && !next.full()) {
-      ks.hide(next.word);
-      vs.hide(next.word);
-    }
+  auto put = [&](char* to, int k0) {
+    next.settle(mb, k0, kend);
+    if (mb && !next.full()) vs.hide(next.word);  // a masked key's scores are replaced, its V would still meet a probability of 0
     ks.put(to);
     vs.put(to + TILE);
     now = next;
   };
-  // one tile: `all` = every key visible to every row of the wave
-  auto step = [&](const char* kt, int k0, auto all) {
-    constexpr bool ALL = decltype(all)::value;
-    const char* vt = kt + TILE;
-    f32x16 sc[SUB];
-#pragma unroll
-    for (int s = 0; s < SUB; ++s) {
-      clear(sc[s]);
-#pragma unroll
-      for (int t = 0; t < NS; ++t) sc[s] = mma(Tile<T, W>::rows(kt, 32 * (wk * SUB + s), t, lane), qf.f[t], sc[s]);
-    }
-    float tmax = -INFINITY;
-#pragma unroll
-    for (int s = 0; s < SUB; ++s) {
-      if constexpr (!ALL) {
-        const int at = 32 * (wk * SUB + s);
-        const unsigned see = (now.of(at) & (a.causal ? bits_to(query + past - k0 - at) : ~0u)) >> (4 * half);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sc[s][i] = see >> acc_row(i) & 1 ? sc[s][i] : -INFINITY;
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, sc[s][i]);
-    }
-    tmax = half_max(tmax) * a.c;
-    if (__any(tmax > m + LAZY)) {
-      const float mn = fmaxf(m, tmax), f = __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      l *= f;
-#pragma unroll
-      for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[dt][i] *= f;
-    }
-#pragma unroll
-    for (int s = 0; s < SUB; ++s) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sc[s][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[s][i], a.c, -m));
-#pragma unroll
-      for (int t = 0; t < TS; ++t) {
-        const auto p = pack_step<T>(sc[s], t);
-#pragma unroll
-        for (int dt = 0; dt < ND; ++dt) o[dt] = mma(Tile<T, W>::transposed(vt, 32 * (wk * SUB + s), t, 32 * dt, lane), p, o[dt]);
-      }
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sum += sc[s][i];
-      l += sum;
-    }
-  };
-
   int at = 0;
   if (kbeg < kend) {
     fetch(kbeg);
-    put(lds);
+    put(lds, kbeg);
     if (NB == 2 && kbeg + KT < kend) fetch(kbeg + KT);
     __syncthreads();
   }
+  // One version of the loop's body, conditions around single steps only: the accumulators stay where they are (with a version for whole tiles
+  // beside one for masked ones the compiler copied them every tile, waiting for the products to do so: 226 us against ...).
   for (int k0 = kbeg; k0 < kend; k0 += KT) {
     if (NB == 1 && k0 + KT < kend) fetch(k0 + KT);
-    unsigned any = 0;
+    const char *kt = lds + at, *vt = kt + TILE;
+    place.afresh();
 #pragma unroll
-    for (int s = 0; s < SUB; ++s) any |= now.of(32 * (wk * SUB + s));
-    if (any && !(a.causal && last_query + past < k0 + 32 * wk * SUB)) {
-      if (now.full() && !(a.causal && first_query + past < k0 + KT - 1))
-        step(lds + at, k0, std::true_type());
-      else
-        step(lds + at, k0, std::false_type());
+    for (int s0 = 0; s0 < SUB; s0 += JOINT) {
+      const int j0 = 32 * (wk * SUB + s0);  // of the tile's keys
+      unsigned any = 0;
+#pragma unroll
+      for (int s = 0; s < JOINT; ++s) any |= now.of(j0 + 32 * s);
+      if (any == 0 || (a.causal && last_query + past < k0 + j0)) continue;
+      f32x16 sc[JOINT][R];
+#pragma unroll
+      for (int s = 0; s < JOINT; ++s) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) clear(sc[s][r]);
+#pragma unroll
+        for (int t = 0; t < NS; ++t) {
+          const auto k = Tile<T, W>::rows(kt, j0 + 32 * s, t, place);
+#pragma unroll
+          for (int r = 0; r < R; ++r) sc[s][r] = mma(k, qf[r].f[t], sc[s][r]);
+        }
+      }
+      if (!now.full() || (a.causal && first_query + past < k0 + j0 + 32 * JOINT - 1)) {
+#pragma unroll
+        for (int s = 0; s < JOINT; ++s)
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const unsigned see = (now.of(j0 + 32 * s) & (a.causal ? bits_to(query[r] + past - k0 - j0 - 32 * s) : ~0u)) >> (4 * half);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[s][r][i] = see >> acc_row(i) & 1 ? sc[s][r][i] : -INFINITY;
+          }
+      }
+      float tmax[R];
+      bool rise = false;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        tmax[r] = -INFINITY;
+#pragma unroll
+        for (int s = 0; s < JOINT; ++s)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) tmax[r] = fmaxf(tmax[r], sc[s][r][i]);
+        tmax[r] = half_max(tmax[r]) * a.c;
+        rise = rise || tmax[r] > m[r] + LAZY;
+      }
+      if (__any(rise)) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float mn = fmaxf(m[r], tmax[r]), f = __builtin_amdgcn_exp2f(m[r] - mn);
+          m[r] = mn;
+          l[r] *= f;
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[r][dt][i] *= f;
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < JOINT; ++s) {
+        typename Elem<T>::Frag p[R][TS];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[s][r][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[s][r][i], a.c, -m[r]));
+#pragma unroll
+          for (int t = 0; t < TS; ++t) p[r][t] = pack_step<T>(sc[s][r], t);
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum += sc[s][r][i];
+          l[r] += sum;
+        }
+#pragma unroll
+        for (int t = 0; t < TS; ++t)
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) {
+            const auto v = Tile<T, W>::transposed(vt, j0 + 32 * s, t, 32 * dt, place);
+#pragma unroll
+            for (int r = 0; r < R; ++r) o[r][dt] = mma(v, p[r][t], o[r][dt]);
+          }
+      }
     }
     if (k0 + KT < kend) {
       if (NB == 1) __syncthreads();
       if (NB == 2) at = 2 * TILE - at;
-      put(lds + at);
+      put(lds + at, k0 + KT);
       if (NB == 2 && k0 + 2 * KT < kend) fetch(k0 + 2 * KT);
       __syncthreads();
     }
   }
-  l = half_sum(l);
+#pragma unroll
+  for (int r = 0; r < R; ++r) l[r] = half_sum(l[r]);
 
   if constexpr (WK > 1) {  // join the waves along the keys in LDS: [wk][32 rows][W + 4], and their (m, l)
-    float *os = reinterpret_cast<float*>(lds), *ml = os + WK * 32 * (W + 4);
+    static_assert(R == 1, "");
+    float *os = reinterpret_cast<float*>(lds), *ml = os + (WK - 1) * 32 * (W + 4), *mine = os + ((wk - 1) * 32 + (lane & 31)) * (W + 4) + 4 * half;
     __syncthreads();
-    if (half == 0) ml[(wk * 32 + (lane & 31)) * 2] = m, ml[(wk * 32 + (lane & 31)) * 2 + 1] = l;
+    if (half == 0) ml[(wk * 32 + (lane & 31)) * 2] = m[0], ml[(wk * 32 + (lane & 31)) * 2 + 1] = l[0];
+    if (wk) {
 #pragma unroll
-    for (int dt = 0; dt < ND; ++dt)
+      for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<float4*>(os + (wk * 32 + (lane & 31)) * (W + 4) + 32 * dt + 8 * q + 4 * half) =
-            make_float4(o[dt][4 * q], o[dt][4 * q + 1], o[dt][4 * q + 2], o[dt][4 * q + 3]);
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<float4*>(mine + 32 * dt + 8 * q) = make_float4(o[0][dt][4 * q], o[0][dt][4 * q + 1], o[0][dt][4 * q + 2], o[0][dt][4 * q + 3]);
+    }
     __syncthreads();
     if (wk) return;
-    float mm = m, f[WK];
+    float mm = m[0], f[WK];
 #pragma unroll
     for (int x = 1; x < WK; ++x) mm = fmaxf(mm, ml[(x * 32 + (lane & 31)) * 2]);
-    l = 0.f;
+    l[0] = 0.f;
 #pragma unroll
     for (int x = 0; x < WK; ++x) {
       f[x] = __builtin_amdgcn_exp2f(ml[(x * 32 + (lane & 31)) * 2] - mm);
-      l += f[x] * ml[(x * 32 + (lane & 31)) * 2 + 1];
+      l[0] += f[x] * ml[(x * 32 + (lane & 31)) * 2 + 1];
     }
-    m = mm;
+    m[0] = mm;
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        float4 v = make_float4(o[dt][4 * q] * f[0], o[dt][4 * q + 1] * f[0], o[dt][4 * q + 2] * f[0], o[dt][4 * q + 3] * f[0]);
+        f32x16& c = o[0][dt];
+        float4 v = make_float4(c[4 * q] * f[0], c[4 * q + 1] * f[0], c[4 * q + 2] * f[0], c[4 * q + 3] * f[0]);
 #pragma unroll
         for (int x = 1; x < WK; ++x) {
-          const float4 u = *reinterpret_cast<const float4*>(os + (x * 32 + (lane & 31)) * (W + 4) + 32 * dt + 8 * q + 4 * half);
+          const float4 u = *reinterpret_cast<const float4*>(os + ((x - 1) * 32 + (lane & 31)) * (W + 4) + 32 * dt + 8 * q + 4 * half);
           v.x += f[x] * u.x, v.y += f[x] * u.y, v.z += f[x] * u.z, v.w += f[x] * u.w;
         }
-        o[dt][4 * q] = v.x, o[dt][4 * q + 1] = v.y, o[dt][4 * q + 2] = v.z, o[dt][4 * q + 3] = v.w;
+        c[4 * q] = v.x, c[4 * q + 1] = v.y, c[4 * q + 2] = v.z, c[4 * q + 3] = v.w;
       }
   }
-  if (row >= a.rows) return;
-  const int g = row - query * a.G, h = w.hk * a.G + g;
-  if (part) {  // one of several splits: unnormalised sums and (m, l), joined by mha_fwd_join
-    const long R = (long)a.B * a.H * a.Lq, r = (w.b * a.Lq + query) * a.H + h;
-    store_row<float, ND>(part + (w.split * R + r) * a.D, o, 1.f, a.D, lane);
-    if (half == 0) {
-      float* ml = part + a.nsplit * R * a.D + (w.split * R + r) * 2;
-      ml[0] = m, ml[1] = l;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (row + 32 * r >= a.rows) break;
+    const int h = w.hk * a.G + row + 32 * r - query[r] * a.G;
+    const long at = (w.b * a.Lq + query[r]) * a.H + h;
+    if (part) {  // one of several splits: unnormalised sums and (m, l), joined by mha_fwd_join
+      const long n = (long)a.B * a.H * a.Lq;
+      store_row<float, ND>(part + (w.split * n + at) * a.D, o[r], 1.f, a.D, lane);
+      if (half == 0) {
+        float* ml = part + a.nsplit * n * a.D + (w.split * n + at) * 2;
+        ml[0] = m[r], ml[1] = l[r];
+      }
+    } else {
+      store_row<T, ND>(out + at * a.D, o[r], l[r] == 0.f ? 0.f : 1.f / l[r], a.D, lane);
+      if (lse && half == 0) lse[(w.b * a.H + h) * a.Lq + query[r]] = l[r] == 0.f ? INFINITY : m[r] + log2f(l[r]);
     }
-    return;
   }
-  store_row<T, ND>(out + ((w.b * a.Lq + query) * a.H + h) * a.D, o, l == 0.f ? 0.f : 1.f / l, a.D, lane);
-  if (lse && half == 0) lse[(w.b * a.H + h) * a.Lq + query] = l == 0.f ? INFINITY : m + log2f(l);
 }
 
 // the splits of a row: a wave per row
@@ -208,14 +250,16 @@ __global__ __launch_bounds__(256) void mha_fwd_join(const float* __restrict__ pa
 
 Plan plan_fwd(int B, int Lq, int Lk, int H, int Hkv) { return plan((long)B * Hkv, Lq * (H / Hkv), Lk); }
 
-template <typename T, int DK, int WQ, int WK, int SUB>
+template <typename T, int DK, int WQ, int R, int WK, int SUB, int JOINT>
 int launch_fwd(const MhaArgs& a, T* out, float* lse, float* part, hipStream_t st) {
   using S = Shape<T, DK>;
-  const size_t tiles = 2 * 32 * WK * SUB * S::ROW, join = WK > 1 ? (size_t)WK * 32 * (S::W + 4 + 2) * 4 : 0;
+  const size_t join = WK > 1 ? (size_t)((WK - 1) * 32 * (S::W + 4) + WK * 32 * 2) * 4 : 0;
+  const size_t tiles = 2 * 32 * WK * SUB * S::ROW;
   size_t lds = 2 * tiles <= 64 * 1024 ? 2 * tiles : tiles;
   if (join > lds) lds = join;
-  if (int rc = prepare_launch(a, mha_fwd_kernel<T, DK, WQ, WK, SUB>, 64 * WQ * WK, lds)) return rc;
-  hipLaunchKernelGGL((mha_fwd_kernel<T, DK, WQ, WK, SUB>), dim3((unsigned)((long)a.B * a.Hkv * a.nblk * a.nsplit)), dim3(64 * WQ * WK), lds, st, a, out, lse, part);
+  const auto kernel = mha_fwd_kernel<T, DK, WQ, R, WK, SUB, JOINT>;
+  if (int rc = prepare_launch(a, kernel, 64 * WQ * WK, lds)) return rc;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((long)a.B * a.Hkv * a.nblk * a.nsplit)), dim3(64 * WQ * WK), lds, st, a, out, lse, part);
   TATT_LAUNCH_CHECK("mha_fwd");
   return TATT_OK;
 }
@@ -226,7 +270,20 @@ int run_fwd(MhaArgs& a, T* out, float* lse, float* part, hipStream_t st) {
   const Plan p = plan_fwd(a.B, a.Lq, a.Lk, a.H, a.Hkv);
   a.nblk = p.nblk, a.nsplit = p.nsplit, a.per_split = p.per_split;
   if (p.nsplit == 1) part = nullptr;
-  if (int rc = p.wide ? launch_fwd<T, DK, 4, 1, 2>(a, out, lse, part, st) : launch_fwd<T, DK, 1, S::WK, 1>(a, out, lse, part, st)) return rc;
+  int rc;
+  if (!p.wide) {
+    rc = launch_fwd<T, DK, 1, 1, S::WK, 1, 1>(a, out, lse, part, st);
+  } else if constexpr (sizeof(T) == 2 && DK <= 64) {
+    if ((long)a.B * a.Hkv * a.nsplit * cdiv(a.rows, 256) >= R2MIN) {
+      a.nblk = cdiv(a.rows, 256);
+      rc = launch_fwd<T, DK, 4, 2, 1, 2, JT>(a, out, lse, part, st);
+    } else {
+      rc = launch_fwd<T, DK, 4, 1, 1, 2, SB>(a, out, lse, part, st);
+    }
+  } else {
+    rc = launch_fwd<T, DK, 4, 1, 1, 2, SB>(a, out, lse, part, st);
+  }
+  if (rc) return rc;
   if (part) {
     const long R = (long)a.B * a.H * a.Lq;
     hipLaunchKernelGGL(mha_fwd_join<T>, dim3(cdiv(R, 4)), dim3(256), 0, st, part, a.nsplit, R, a.D, a.H, a.Lq, out, lse);

@@ -49,6 +49,11 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _like(t):
+    """A contiguous tensor of t's shape, type and device."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _rows(t):
     """t with a contiguous last dimension (a copy only if it has none)."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
@@ -80,9 +85,9 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None, need_
     _parameters("layer_norm", x, weight, bias)
     C = x.shape[-1]
     R = x.numel() // C
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    s = torch.empty_like(y) if residual is not None else x
-    stat = torch.empty(R, 2, dtype=torch.float32, device=x.device) if need_stat else None
+    y = _like(x)
+    s = _like(x) if residual is not None else x
+    stat = torch.empty((R, 2), dtype=torch.float32, device=x.device) if need_stat else None
     if R:
         xm, ldx = _matrix(x)
         rm, ldr = (None, 0) if residual is None else _matrix(residual)
@@ -100,8 +105,10 @@ def layer_norm_backward(dy, s, weight, stat, dsum=None, need_params=True):
     R = s.numel() // C
     if dy.shape != s.shape or (dsum is not None and dsum.shape != s.shape) or stat.shape != (R, 2) or stat.dtype != torch.float32 or stat.device != s.device or not stat.is_contiguous():
         raise RuntimeError("tatt_amd layer_norm_backward: dy and dsum have the shape of the sum, stat is layer_norm_forward's")
-    ds = torch.empty(s.shape, dtype=s.dtype, device=s.device)
-    dw, db = (torch.empty(2, C, dtype=torch.float32, device=s.device) if R else torch.zeros(2, C, device=s.device)).unbind() if need_params else (None, None)
+    ds, dw, db = _like(s), None, None
+    if need_params:
+        new = torch.empty if R else torch.zeros
+        dw, db = (new(C, dtype=torch.float32, device=s.device) for _ in range(2))
     if R:
         sm, lds = _matrix(s)
         dym, lddy = _matrix(dy)
@@ -161,8 +168,7 @@ def rotate(q, k, positions, freqs, sections, interleaved=False, inverse=False):
         raise RuntimeError(f"tatt_amd rotary: positions [L, axes] or [B, L, axes] on the tensors' device expected, got {tuple(positions.shape)} on {positions.device}")
     if freqs.dtype != torch.float64 or freqs.shape != (sum(sections) // 2,) or freqs.device != q.device or not freqs.is_contiguous():
         raise RuntimeError("tatt_amd rotary: freqs is a contiguous float64 vector of sum(sections) / 2 on the tensors' device (rotary_frequencies)")
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    qo, ko = _like(q), None if k is None else _like(k)
     if qo.numel():
         q, k = _rows(q), None if k is None or not k.numel() else _rows(k)
         sp = positions.stride()
@@ -243,8 +249,8 @@ def attention_forward(q, k, v, key_padding_mask=None, causal=False, scale=None, 
     q, k, v = _laid_out(q, dtype, H // Hk), _laid_out(k, dtype), _laid_out(v, dtype)
     P = q.shape[3]
     dims = (B, Lq, Lk, H, Hk, P)
-    out = torch.empty(B, Lq, H, P, dtype=q.dtype, device=q.device)
-    lse = torch.empty(B, H, Lq, dtype=torch.float32, device=q.device) if need_lse else None
+    out = _like(q)
+    lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device) if need_lse else None
     n = lib().cdll.tatt_mha_fwd_workspace(*dims, dtype)
     ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
     mask_strides = None if key_padding_mask is None else _L2(*key_padding_mask.stride())
@@ -266,8 +272,7 @@ def attention_backward(dout, q, k, v, out, lse, key_padding_mask=None, causal=Fa
     k, v = _laid_out(k, dtype), _laid_out(v, dtype)
     P = q.shape[3]
     dims = (B, Lq, Lk, H, Hk, P)
-    dq = torch.empty(B, Lq, H, P, dtype=q.dtype, device=q.device)
-    dk, dv = torch.empty(2, B, Lk, Hk, P, dtype=q.dtype, device=q.device).unbind()
+    dq, dk, dv = _like(q), _like(k), _like(v)
     ws = torch.empty(lib().cdll.tatt_mha_bwd_workspace(*dims, dtype), dtype=torch.float32, device=q.device)
     mask_strides = None if key_padding_mask is None else _L2(*key_padding_mask.stride())
     _call("tatt_mha_bwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(),
