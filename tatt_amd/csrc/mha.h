@@ -21,18 +21,6 @@
 #pragma once
 #include "token_types.h"
 
-#ifndef FW
-#define FW 2
-#endif
-#ifndef DQ
-#define DQ 2
-#endif
-#ifndef DKV128
-#define DKV128 1
-#endif
-#ifndef DKV
-#define DKV 2
-#endif
 namespace {
 
 __device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
@@ -57,13 +45,13 @@ __device__ __forceinline__ typename Elem<T>::Frag pack_step(const f32x16& c, int
 }
 
 // waves a SIMD that the registers are shared out for.  Two (256 registers each) unless what a wave has to hold -- the fragments of its rows, the
-// sums, a tile on its way -- would spill: then one, the sums in the other half of the register file.
+// sums, a tile on its way -- would spill: then one (dK and dV of 128 in bf16: 384 us with two and 187 spilled registers, 230 with one).
 template <typename T>
-constexpr int fwd_waves(int DK) { return sizeof(T) == 4 && DK > 64 ? 1 : DK <= 64 ? FW : 2; }
+constexpr int fwd_waves(int DK) { return sizeof(T) == 4 && DK > 64 ? 1 : 2; }
 template <typename T>
-constexpr int dq_waves(int DK) { return sizeof(T) == 4 && DK >= 64 ? 1 : DK <= 64 ? DQ : 2; }
+constexpr int dq_waves(int DK) { return sizeof(T) == 4 && DK >= 64 ? 1 : 2; }
 template <typename T>
-constexpr int dkv_waves(int DK) { return (DK > 64 && DKV128) || (sizeof(T) == 4 && DK == 64) ? 1 : DKV; }
+constexpr int dkv_waves(int DK) { return DK > 64 || (sizeof(T) == 4 && DK == 64) ? 1 : 2; }
 
 // head widths the kernels are built for, and the LDS row that holds one
 constexpr int row_width(int DK) { return DK <= 32 ? 32 : DK <= 64 ? 64 : 128; }
@@ -148,10 +136,12 @@ struct Where {
   int blk, split, hk;
   long b;
 };
-// Workgroups go round the 8 XCDs in turn; each XCD gets a contiguous range of the work, so that the blocks that read one key head share an L2.
+// Workgroups go round the 8 XCDs in turn.  Each XCD gets a contiguous range of the work, so that the blocks that read one key head share an L2
+// (fp32, 16 x 4 heads of 1024: 2-6 % faster) -- but not where the work of a range may differ: with a mask (sequences of different lengths; two
+// clips, one of them empty: dK and dV in 335 us against 243) or with splits, which share nothing.
 __device__ __forceinline__ Where where(const MhaArgs& a) {
   const unsigned n = gridDim.x, per = n / 8, rest = n % 8, x = blockIdx.x % 8, y = blockIdx.x / 8;
-  unsigned id = x * per + min(x, rest) + y;
+  unsigned id = a.mask || a.nsplit > 1 ? blockIdx.x : x * per + min(x, rest) + y;
   Where w;
   w.blk = id % a.nblk;
   id /= a.nblk;
@@ -276,6 +266,33 @@ struct KeyBits {
   __device__ __forceinline__ unsigned of(int at) const { return (unsigned)(word[at / 64] >> (at & 63)); }  // 32 keys from `at` on
 };
 
+// [lo, hi) shrunk to its first and last key that is not masked (padding at a sequence's end is not even read); `red` = 8 bytes of LDS a wave
+template <int NT>
+__device__ __forceinline__ void trim_keys(const unsigned char* mask, long stride, int& lo, int& hi, int* red) {
+  int first = hi, last = lo - 1;
+#pragma unroll 4
+  for (int j = lo + (int)threadIdx.x; j < hi; j += NT)
+    if (!mask[j * stride]) {
+      first = min(first, j);
+      last = max(last, j);
+    }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    first = min(first, __shfl_xor(first, o, 64));
+    last = max(last, __shfl_xor(last, o, 64));
+  }
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = first, red[NT / 64 + (threadIdx.x >> 6)] = last;
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < NT / 64; ++x) {
+    first = min(first, red[x]);
+    last = max(last, red[NT / 64 + x]);
+  }
+  __syncthreads();
+  lo = __builtin_amdgcn_readfirstlane(first);
+  hi = __builtin_amdgcn_readfirstlane(last + 1);
+}
+
 // the D elements of one row held as accumulators of a transposed product (lane = row, registers = dimensions), times f, to dst
 template <typename T, int ND>
 __device__ __forceinline__ void store_row(T* dst, const f32x16 (&o)[ND], float f, int D, int lane) {
@@ -313,6 +330,10 @@ __device__ __forceinline__ void clear(f32x16 (&o)[N]) {
 #pragma unroll
   for (int n = 0; n < N; ++n) clear(o[n]);
 }
+
+// Waits for every load issued so far.  Once before a loop: the fragments loaded for it are then known to be there, and their first use inside the
+// loop does not wait for the tile that is on its way (which exposed the whole latency of global memory every iteration).
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }  // vmcnt(0)
 
 // bits 0 .. n (n < 0: none, n >= 31: all)
 __device__ __forceinline__ unsigned bits_to(int n) { return n < 0 ? 0u : n >= 31 ? ~0u : (2u << n) - 1u; }
@@ -388,7 +409,6 @@ int prepare_launch(const MhaArgs& a, K kernel, int threads, size_t bytes) {
 template <typename T, int DK>
 struct Shape {
   static constexpr int W = row_width(DK), ROW = Tile<T, W>::ROW;
-  static constexpr int WKF = ROW > 256 ? 1 : ROW == 256 ? 2 : 4;  // forward: four tiles of 32 WK rows within 64 KB
   static constexpr int WK = ROW > 256 ? 2 : 4;  // waves along the summed axis: two tiles of 32 WK rows within 64 KB
 };
 

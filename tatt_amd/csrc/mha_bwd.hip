@@ -3,13 +3,10 @@
 // are keys (dK, dV): seven products instead of the five that atomics into dQ would need, and sums in a fixed order.
 #include "mha.h"
 
-#ifndef DQSUB
-#define DQSUB 1
-#endif
 namespace {
 
-// dQ and delta.  WQ waves of 32 rows; registers hold Q and dO, LDS tiles of 32 SUB keys K and V.
-template <typename T, int DK, int WQ, int SUB>
+// dQ and delta.  WQ waves of 32 R rows; registers hold Q and dO, LDS tiles of 32 SUB keys K and V.
+template <typename T, int DK, int WQ, int R, int SUB>
 __global__ __launch_bounds__(64 * WQ, dq_waves<T>(DK)) void mha_dq_kernel(MhaArgs a, T* __restrict__ dq, float* __restrict__ part) {
   constexpr int NT = 64 * WQ, W = row_width(DK), ND = (DK + 31) / 32, KT = 32 * SUB, TILE = KT * Tile<T, W>::ROW;
   constexpr int NS = DK / Elem<T>::STEP, TS = 32 / Elem<T>::STEP, NB = 4 * TILE <= 64 * 1024 ? 2 : 1;
@@ -17,42 +14,48 @@ __global__ __launch_bounds__(64 * WQ, dq_waves<T>(DK)) void mha_dq_kernel(MhaArg
   const int lane = threadIdx.x & 63, wq = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const Where w = where(a);
   const int blk = a.causal ? a.nblk - 1 - w.blk : w.blk;
-  const int row0 = blk * 32 * WQ, row = row0 + 32 * wq + (lane & 31), past = a.Lk - a.Lq;
-  const bool on = row < a.rows;
-  const int safe = min(row, a.rows - 1), query = (unsigned)safe / (unsigned)a.G, h = w.hk * a.G + safe - query * a.G;
-  const int first_query = (row0 + 32 * wq) / a.G, last_query = min(a.rows - 1, row0 + 32 * wq + 31) / a.G;
+  const int row0 = blk * 32 * WQ * R, wrow0 = row0 + 32 * wq * R, row = wrow0 + (lane & 31), past = a.Lk - a.Lq;  // and row + 32 r
+  const int first_query = wrow0 / a.G;
   const T* kb = (const T*)a.k + w.b * a.ks[0] + w.hk * a.ks[2];
   const T* vb = (const T*)a.v + w.b * a.vs[0] + w.hk * a.vs[2];
   const unsigned char* mb = a.mask ? a.mask + w.b * a.mask_sb : nullptr;
 
-  RowFrags<T, DK> qf, gf;
-  qf.load((const T*)a.q + w.b * a.qs[0] + query * a.qs[1] + h * a.qs[2], on, a.D, lane);
-  gf.load((const T*)a.dout + w.b * a.dos[0] + query * a.dos[1] + h * a.dos[2], on, a.D, lane);
-  if (a.scale < 0.f) qf.negate();
-  float delta = 0.f;
-  {
-    const T* orow = (const T*)a.out + w.b * a.os[0] + query * a.os[1] + h * a.os[2];
+  RowFrags<T, DK> qf[R], gf[R];
+  int query[R];
+  long at_row[R];  // row of dQ
+  float lse[R], delta[R];
+  f32x16 o[R][ND];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const bool on = row + 32 * r < a.rows;
+    const int safe = min(row + 32 * r, a.rows - 1);
+    query[r] = (unsigned)safe / (unsigned)a.G;
+    const int h = w.hk * a.G + safe - query[r] * a.G;
+    at_row[r] = (w.b * a.Lq + query[r]) * a.H + h;
+    qf[r].load((const T*)a.q + w.b * a.qs[0] + query[r] * a.qs[1] + h * a.qs[2], on, a.D, lane);
+    gf[r].load((const T*)a.dout + w.b * a.dos[0] + query[r] * a.dos[1] + h * a.dos[2], on, a.D, lane);
+    if (a.scale < 0.f) qf[r].negate();
+    const T* orow = (const T*)a.out + w.b * a.os[0] + query[r] * a.os[1] + h * a.os[2];
+    float d = 0.f;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       const uint4 u = load_chunk<T>(orow, 2 * s + half, a.D, 1);
       T t[Elem<T>::PER_CHUNK];
       memcpy(t, &u, 16);
 #pragma unroll
-      for (int e = 0; e < Elem<T>::PER_CHUNK; ++e) delta += to_f32(t[e]) * (float)gf.f[s][e];
+      for (int e = 0; e < Elem<T>::PER_CHUNK; ++e) d += to_f32(t[e]) * (float)gf[r].f[s][e];
     }
-    delta = half_sum(delta);
+    const long stat = (w.b * a.H + h) * a.Lq + query[r];
+    lse[r] = on ? a.lse[stat] : INFINITY;
+    delta[r] = lse[r] == INFINITY ? 0.f : half_sum(d);  // a row that sees nothing: whatever dO holds there
+    if (on && half == 0 && w.split == 0) a.delta[stat] = delta[r];
+    clear(o[r]);
   }
-  const long stat = (w.b * a.H + h) * a.Lq + query;
-  const float lse = on ? a.lse[stat] : INFINITY;
-  const bool empty = lse == INFINITY;
-  if (empty) delta = 0.f;  // whatever dO holds there
-  if (on && half == 0 && w.split == 0) a.delta[stat] = delta;
 
-  const int kbeg = w.split * a.per_split;
+  int kbeg = w.split * a.per_split;
   int kend = min(a.Lk, kbeg + a.per_split);
-  if (a.causal) kend = min(kend, min(a.rows - 1, row0 + 32 * WQ - 1) / a.G + past + 1);
-  f32x16 o[ND];
-  clear(o);
+  if (a.causal) kend = min(kend, min(a.rows - 1, row0 + 32 * WQ * R - 1) / a.G + past + 1);
+  if (mb && kend - kbeg > 2 * KT) trim_keys<NT>(mb, a.mask_sl, kbeg, kend, reinterpret_cast<int*>(lds));
   Stage<T, W, KT, NT, true> ks, vs;
   KeyBits<KT> next, now;
   ks.linear(a.ks[1], a.D);
@@ -74,6 +77,7 @@ __global__ __launch_bounds__(64 * WQ, dq_waves<T>(DK)) void mha_dq_kernel(MhaArg
   if (kbeg < kend) {
     fetch(kbeg);
     put(lds, kbeg);
+    wait_loads();
     if (NB == 2 && kbeg + KT < kend) fetch(kbeg + KT);
     __syncthreads();
   }
@@ -83,27 +87,49 @@ __global__ __launch_bounds__(64 * WQ, dq_waves<T>(DK)) void mha_dq_kernel(MhaArg
     place.afresh();
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
-      if (now.of(32 * s) == 0 || (a.causal && last_query + past < k0 + 32 * s)) continue;
-      f32x16 sc, dp;
-      clear(sc);
-      clear(dp);
+      f32x16 sc[R], dp[R];
 #pragma unroll
-      for (int t = 0; t < NS; ++t) sc = mma(Tile<T, W>::rows(kt, 32 * s, t, place), qf.f[t], sc);
+      for (int r = 0; r < R; ++r) {
+        clear(sc[r]);
+        clear(dp[r]);
+      }
 #pragma unroll
-      for (int t = 0; t < NS; ++t) dp = mma(Tile<T, W>::rows(vt, 32 * s, t, place), gf.f[t], dp);
+      for (int t = 0; t < NS; ++t) {
+        const auto k = Tile<T, W>::rows(kt, 32 * s, t, place);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], a.c, -lse)) * (dp[i] - delta);
+        for (int r = 0; r < R; ++r) sc[r] = mma(k, qf[r].f[t], sc[r]);
+      }
+#pragma unroll
+      for (int t = 0; t < NS; ++t) {
+        const auto v = Tile<T, W>::rows(vt, 32 * s, t, place);
+#pragma unroll
+        for (int r = 0; r < R; ++r) dp[r] = mma(v, gf[r].f[t], dp[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[r][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][i], a.c, -lse[r])) * (dp[r][i] - delta[r]);
       if (!now.full() || (a.causal && first_query + past < k0 + 32 * s + 31)) {
-        const unsigned see = (now.of(32 * s) & (a.causal ? bits_to(query + past - k0 - 32 * s) : ~0u)) >> (4 * half);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sc[i] = see >> acc_row(i) & 1 ? sc[i] : 0.f;
+        for (int r = 0; r < R; ++r) {
+          const unsigned see = (now.of(32 * s) & (a.causal ? bits_to(query[r] + past - k0 - 32 * s) : ~0u)) >> (4 * half);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[r][i] = see >> acc_row(i) & 1 ? sc[r][i] : 0.f;
+        }
       }
+      typename Elem<T>::Frag p[R][TS];
 #pragma unroll
-      for (int t = 0; t < TS; ++t) {
-        const auto p = pack_step<T>(sc, t);
+      for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int dt = 0; dt < ND; ++dt) o[dt] = mma(Tile<T, W>::transposed(kt, 32 * s, t, 32 * dt, place), p, o[dt]);
-      }
+        for (int t = 0; t < TS; ++t) p[r][t] = pack_step<T>(sc[r], t);
+#pragma unroll
+      for (int t = 0; t < TS; ++t)
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) {
+          const auto k = Tile<T, W>::transposed(kt, 32 * s, t, 32 * dt, place);
+#pragma unroll
+          for (int r = 0; r < R; ++r) o[r][dt] = mma(k, p[r][t], o[r][dt]);
+        }
     }
     if (k0 + KT < kend) {
       if (NB == 1) __syncthreads();
@@ -113,19 +139,21 @@ __global__ __launch_bounds__(64 * WQ, dq_waves<T>(DK)) void mha_dq_kernel(MhaArg
       __syncthreads();
     }
   }
-  if (!on) return;
-  if (empty) clear(o);
-  const long r = (w.b * a.Lq + query) * a.H + h;
-  if (part)
-    store_row<float, ND>(part + (w.split * (long)a.B * a.H * a.Lq + r) * a.D, o, a.scale, a.D, lane);
-  else
-    store_row<T, ND>(dq + r * a.D, o, a.scale, a.D, lane);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (row + 32 * r >= a.rows) break;
+    if (lse[r] == INFINITY) clear(o[r]);
+    if (part)
+      store_row<float, ND>(part + (w.split * (long)a.B * a.H * a.Lq + at_row[r]) * a.D, o[r], a.scale, a.D, lane);
+    else
+      store_row<T, ND>(dq + at_row[r] * a.D, o[r], a.scale, a.D, lane);
+  }
 }
 
-// dK and dV.  WN waves along the keys (32 each) x WR along the rows; LDS holds tiles of 32 WR rows of Q and dO, and their lse and delta.
-template <typename T, int DK, int WN, int WR>
+// dK and dV.  WN waves along the keys (32 each) x WR along the rows; LDS holds tiles of 32 WR SUB rows of Q and dO, and their lse and delta.
+template <typename T, int DK, int WN, int WR, int SUB>
 __global__ __launch_bounds__(64 * WN * WR, dkv_waves<T>(DK)) void mha_dkv_kernel(MhaArgs a, T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part) {
-  constexpr int NT = 64 * WN * WR, W = row_width(DK), ND = (DK + 31) / 32, RT = 32 * WR, TILE = RT * Tile<T, W>::ROW, BUF = 2 * TILE + 2 * RT * 4;
+  constexpr int NT = 64 * WN * WR, W = row_width(DK), ND = (DK + 31) / 32, RT = 32 * WR * SUB, TILE = RT * Tile<T, W>::ROW, BUF = 2 * TILE + 2 * RT * 4;
   constexpr int NS = DK / Elem<T>::STEP, TS = 32 / Elem<T>::STEP, NB = 4 * TILE <= 64 * 1024 ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wr = wave / WN, half = lane >> 5;
@@ -145,7 +173,6 @@ __global__ __launch_bounds__(64 * WN * WR, dkv_waves<T>(DK)) void mha_dkv_kernel
   // causal: this key is seen from row G (key - past) on; rows before the first query that sees anything hold what they like
   const int first_row = a.causal ? a.G * max(0, key - past) : 0;
   const int all_rows = a.causal ? a.G * max(0, key0 + 32 * wn + 31 - past) : 0;  // from here on every key of the wave is seen
-  const int none_rows = a.causal ? a.G * max(0, key0 + 32 * wn - past) : 0;      // below this none is
   const int empty_rows = a.causal ? a.G * max(0, -past) : 0;
   const bool whole = __all(on);
   int rbeg = w.split * a.per_split;
@@ -169,6 +196,7 @@ __global__ __launch_bounds__(64 * WN * WR, dkv_waves<T>(DK)) void mha_dkv_kernel
     const int i0 = r0 / a.G;
     qs.load(qb + i0 * a.qs[1], empty_rows - r0, rend - r0);
     gs.load(gb + i0 * a.dos[1], empty_rows - r0, rend - r0);
+    static_assert(RT <= NT, "");
     if (threadIdx.x < RT) {
       const int r = r0 + threadIdx.x;
       const bool there = r < rend && r >= empty_rows;
@@ -190,15 +218,17 @@ __global__ __launch_bounds__(64 * WN * WR, dkv_waves<T>(DK)) void mha_dkv_kernel
     if (steady) places(0);
     fetch(rbeg);
     put(lds);
+    wait_loads();
     if (NB == 2 && rbeg + RT < rend) fetch(rbeg + RT);
     __syncthreads();
     for (int r0 = rbeg; r0 < rend; r0 += RT) {
       if (NB == 1 && r0 + RT < rend) fetch(r0 + RT);
-      const int at = 32 * wr;
-      if (r0 + at + 31 >= none_rows) {
-        const char *qt = lds + buf, *gt = qt + TILE;
-        const float* ls = reinterpret_cast<const float*>(qt + 2 * TILE);
-        place.afresh();
+      const char *qt = lds + buf, *gt = qt + TILE;
+      const float* ls = reinterpret_cast<const float*>(qt + 2 * TILE);
+      place.afresh();
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) {
+        const int at = 32 * (wr * SUB + s);
         f32x16 sc, dp;
         clear(sc);
         clear(dp);
@@ -213,9 +243,9 @@ __global__ __launch_bounds__(64 * WN * WR, dkv_waves<T>(DK)) void mha_dkv_kernel
           for (int e = 0; e < 4; ++e) sc[4 * q + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[4 * q + e], a.c, -lq[e]));
         }
         if (!whole || r0 + at < all_rows) {
-          const int hidden = first_row - r0 - at - 4 * half;  // accumulator rows below this are causally hidden
+          const int hidden = on ? first_row - r0 - at - 4 * half : 32;  // accumulator rows below this are causally hidden
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sc[i] = on && acc_row(i) >= hidden ? sc[i] : 0.f;
+          for (int i = 0; i < 16; ++i) sc[i] = acc_row(i) >= hidden ? sc[i] : 0.f;
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -293,14 +323,24 @@ __global__ __launch_bounds__(256) void mha_sum_kernel(const float* __restrict__ 
 Plan plan_dq(int B, int Lq, int Lk, int H, int Hkv) { return plan((long)B * Hkv, Lq * (H / Hkv), Lk); }
 Plan plan_dkv(int B, int Lq, int Lk, int H, int Hkv) { return plan((long)B * Hkv, Lk, Lq * (H / Hkv)); }
 
-template <typename T, int DK, int WN, int WR>
+template <typename T, int DK, int R, int SUB>
+int launch_dq(const MhaArgs& a, T* dq, float* part, hipStream_t st) {
+  const size_t tiles = 2 * 32 * SUB * Shape<T, DK>::ROW, lds = 2 * tiles <= 64 * 1024 ? 2 * tiles : tiles;
+  const auto kernel = mha_dq_kernel<T, DK, 4, R, SUB>;
+  if (int rc = prepare_launch(a, kernel, 256, lds)) return rc;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((long)a.B * a.Hkv * a.nblk * a.nsplit)), dim3(256), lds, st, a, dq, part);
+  TATT_LAUNCH_CHECK("mha_dq");
+  return TATT_OK;
+}
+
+template <typename T, int DK, int WN, int WR, int SUB>
 int launch_dkv(const MhaArgs& a, T* dk, T* dv, float* part, hipStream_t st) {
   using S = Shape<T, DK>;
-  const size_t tiles = 2 * 32 * WR * S::ROW, buf = tiles + 2 * 32 * WR * 4, join = WR > 1 ? (size_t)WN * 32 * (S::W + 4) * 4 : 0;
+  const size_t tiles = 2 * 32 * WR * SUB * S::ROW, buf = tiles + 2 * 32 * WR * SUB * 4, join = WR > 1 ? (size_t)WN * 32 * (S::W + 4) * 4 : 0;
   size_t lds = 2 * tiles <= 64 * 1024 ? 2 * buf : buf;
   if (join > lds) lds = join;
-  if (int rc = prepare_launch(a, mha_dkv_kernel<T, DK, WN, WR>, 64 * WN * WR, lds)) return rc;
-  hipLaunchKernelGGL((mha_dkv_kernel<T, DK, WN, WR>), dim3((unsigned)((long)a.B * a.Hkv * a.nblk * a.nsplit)), dim3(64 * WN * WR), lds, st, a, dk, dv, part);
+  if (int rc = prepare_launch(a, mha_dkv_kernel<T, DK, WN, WR, SUB>, 64 * WN * WR, lds)) return rc;
+  hipLaunchKernelGGL((mha_dkv_kernel<T, DK, WN, WR, SUB>), dim3((unsigned)((long)a.B * a.Hkv * a.nblk * a.nsplit)), dim3(64 * WN * WR), lds, st, a, dk, dv, part);
   TATT_LAUNCH_CHECK("mha_dkv");
   return TATT_OK;
 }
@@ -309,24 +349,26 @@ template <typename T, int DK>
 int run_bwd(MhaArgs& a, T* dq, T* dk, T* dv, float* part, hipStream_t st) {
   using S = Shape<T, DK>;
   Plan p = plan_dq(a.B, a.Lq, a.Lk, a.H, a.Hkv);
-  a.nblk = cdiv(a.rows, 128), a.nsplit = p.nsplit, a.per_split = p.per_split;
-  {
-    constexpr int SUB = DK > 64 ? DQSUB : 2;
-    const size_t tiles = 2 * 32 * SUB * S::ROW, lds = 2 * tiles <= 64 * 1024 ? 2 * tiles : tiles;
-    if (int rc = prepare_launch(a, mha_dq_kernel<T, DK, 4, SUB>, 256, lds)) return rc;
-    hipLaunchKernelGGL((mha_dq_kernel<T, DK, 4, SUB>), dim3((unsigned)((long)a.B * a.Hkv * a.nblk * a.nsplit)), dim3(256), lds, st, a, dq,
-                       a.nsplit > 1 ? part : nullptr);
-    TATT_LAUNCH_CHECK("mha_dq");
-    if (a.nsplit > 1) {
-      const long n = (long)a.B * a.H * a.Lq * a.D;
-      hipLaunchKernelGGL(mha_sum_kernel<T>, dim3(cdiv(n, 256)), dim3(256), 0, st, part, a.nsplit, n, dq, (T*)nullptr);
-      TATT_LAUNCH_CHECK("mha_sum");
-    }
+  a.nsplit = p.nsplit, a.per_split = p.per_split;
+  float* q_part = a.nsplit > 1 ? part : nullptr;
+  int rc;
+  if (sizeof(T) == 2 && DK <= 64 && (long)a.B * a.Hkv * a.nsplit * cdiv(a.rows, 256) >= 256) {
+    a.nblk = cdiv(a.rows, 256);
+    rc = launch_dq<T, DK, (sizeof(T) == 2 && DK <= 64 ? 2 : 1), 2>(a, dq, q_part, st);
+  } else {
+    a.nblk = cdiv(a.rows, 128);
+    rc = launch_dq<T, DK, 1, (DK > 64 && sizeof(T) == 4 ? 1 : 2)>(a, dq, q_part, st);
+  }
+  if (rc) return rc;
+  if (q_part) {
+    const long n = (long)a.B * a.H * a.Lq * a.D;
+    hipLaunchKernelGGL(mha_sum_kernel<T>, dim3(cdiv(n, 256)), dim3(256), 0, st, part, a.nsplit, n, dq, (T*)nullptr);
+    TATT_LAUNCH_CHECK("mha_sum");
   }
   p = plan_dkv(a.B, a.Lq, a.Lk, a.H, a.Hkv);
   a.nblk = p.nblk, a.nsplit = p.nsplit, a.per_split = p.per_split;
   float* kv_part = a.nsplit > 1 ? part : nullptr;
-  if (int rc = p.wide ? launch_dkv<T, DK, 4, 1>(a, dk, dv, kv_part, st) : launch_dkv<T, DK, 1, S::WK>(a, dk, dv, kv_part, st)) return rc;
+  if ((rc = p.wide ? launch_dkv<T, DK, 4, 1, (sizeof(T) == 4 ? 1 : DK > 64 ? 2 : 4)>(a, dk, dv, kv_part, st) : launch_dkv<T, DK, 1, S::WK, 1>(a, dk, dv, kv_part, st))) return rc;
   if (kv_part) {
     const long n = (long)a.B * a.Hkv * a.Lk * a.D;
     hipLaunchKernelGGL(mha_sum_kernel<T>, dim3(cdiv(2 * n, 256)), dim3(256), 0, st, part, a.nsplit, n, dk, dv);

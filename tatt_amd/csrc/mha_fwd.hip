@@ -2,15 +2,6 @@
 // and the layouts).  One pass over the keys with a running maximum and sum; no score leaves the registers.
 #include "mha.h"
 
-#ifndef JT
-#define JT 2
-#endif
-#ifndef SB
-#define SB 2
-#endif
-#ifndef R2MIN
-#define R2MIN 256
-#endif
 namespace {
 
 constexpr float NO_MAX = -1e30f;  // the running maximum before any visible score; finite, so that differences from it are not NaN
@@ -30,7 +21,7 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
   const T* vb = (const T*)a.v + w.b * a.vs[0] + w.hk * a.vs[2];
   const unsigned char* mb = a.mask ? a.mask + w.b * a.mask_sb : nullptr;
   const int past = a.Lk - a.Lq;
-  const int first_query = wrow0 / a.G, last_query = min(a.rows - 1, wrow0 + 32 * R - 1) / a.G;
+  const int first_query = wrow0 / a.G;
 
   RowFrags<T, DK> qf[R];
   int query[R];
@@ -46,9 +37,10 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
     l[r] = 0.f;
   }
 
-  const int kbeg = w.split * a.per_split;
+  int kbeg = w.split * a.per_split;
   int kend = min(a.Lk, kbeg + a.per_split);
   if (a.causal) kend = min(kend, min(a.rows - 1, row0 + 32 * WQ * R - 1) / a.G + past + 1);
+  if (mb && kend - kbeg > 2 * KT) trim_keys<NT>(mb, a.mask_sl, kbeg, kend, reinterpret_cast<int*>(lds));
 
   Stage<T, W, KT, NT, true> ks, vs;
   KeyBits<KT> next, now;
@@ -71,6 +63,7 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
   if (kbeg < kend) {
     fetch(kbeg);
     put(lds, kbeg);
+    wait_loads();
     if (NB == 2 && kbeg + KT < kend) fetch(kbeg + KT);
     __syncthreads();
   }
@@ -83,10 +76,6 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
 #pragma unroll
     for (int s0 = 0; s0 < SUB; s0 += JOINT) {
       const int j0 = 32 * (wk * SUB + s0);  // of the tile's keys
-      unsigned any = 0;
-#pragma unroll
-      for (int s = 0; s < JOINT; ++s) any |= now.of(j0 + 32 * s);
-      if (any == 0 || (a.causal && last_query + past < k0 + j0)) continue;
       f32x16 sc[JOINT][R];
 #pragma unroll
       for (int s = 0; s < JOINT; ++s) {
@@ -225,23 +214,34 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
   }
 }
 
-// the splits of a row: a wave per row
+// the splits of a row: a wave per row, lane = split for the weights, then lane = dimension
 template <typename T>
 __global__ __launch_bounds__(256) void mha_fwd_join(const float* __restrict__ part, int nsplit, long R, int D, int H, int Lq, T* __restrict__ out, float* __restrict__ lse) {
   const int lane = threadIdx.x & 63;
   const long r = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= R) return;
   const float* ml = part + nsplit * R * D;
-  float m = NO_MAX, l = 0.f;
-  for (int s = 0; s < nsplit; ++s) m = fmaxf(m, ml[(s * R + r) * 2]);
-  float o0 = 0.f, o1 = 0.f;
-  for (int s = 0; s < nsplit; ++s) {
-    const float f = __builtin_amdgcn_exp2f(ml[(s * R + r) * 2] - m);
-    l += f * ml[(s * R + r) * 2 + 1];
-    const float* p = part + (s * R + r) * D;
-    if (lane < D) o0 += f * p[lane];
-    if (lane + 64 < D) o1 += f * p[lane + 64];
+  float m = NO_MAX;
+  for (int s = lane; s < nsplit; s += 64) m = fmaxf(m, ml[(s * R + r) * 2]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  float l = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int s0 = 0; s0 < nsplit; s0 += 64) {
+    float f = 0.f;
+    if (s0 + lane < nsplit) {
+      const float2 v = *reinterpret_cast<const float2*>(ml + ((s0 + lane) * R + r) * 2);
+      f = __builtin_amdgcn_exp2f(v.x - m);
+      l += f * v.y;
+    }
+    const int n = min(64, nsplit - s0);
+    for (int s = 0; s < n; ++s) {
+      const float w = __shfl(f, s, 64);
+      const float* p = part + ((s0 + s) * R + r) * D;
+      if (lane < D) o0 += w * p[lane];
+      if (lane + 64 < D) o1 += w * p[lane + 64];
+    }
   }
+  l = wave_sum(l);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   if (lane < D) out[r * D + lane] = from_f32<T>(o0 * inv);
   if (lane + 64 < D) out[r * D + lane + 64] = from_f32<T>(o1 * inv);
@@ -274,14 +274,14 @@ int run_fwd(MhaArgs& a, T* out, float* lse, float* part, hipStream_t st) {
   if (!p.wide) {
     rc = launch_fwd<T, DK, 1, 1, S::WK, 1, 1>(a, out, lse, part, st);
   } else if constexpr (sizeof(T) == 2 && DK <= 64) {
-    if ((long)a.B * a.Hkv * a.nsplit * cdiv(a.rows, 256) >= R2MIN) {
+    if ((long)a.B * a.Hkv * a.nsplit * cdiv(a.rows, 256) >= 256) {
       a.nblk = cdiv(a.rows, 256);
-      rc = launch_fwd<T, DK, 4, 2, 1, 2, JT>(a, out, lse, part, st);
+      rc = launch_fwd<T, DK, 4, 2, 1, 2, 2>(a, out, lse, part, st);
     } else {
-      rc = launch_fwd<T, DK, 4, 1, 1, 2, SB>(a, out, lse, part, st);
+      rc = launch_fwd<T, DK, 4, 1, 1, 2, 2>(a, out, lse, part, st);
     }
   } else {
-    rc = launch_fwd<T, DK, 4, 1, 1, 2, SB>(a, out, lse, part, st);
+    rc = launch_fwd<T, DK, 4, 1, 1, 2, 2>(a, out, lse, part, st);
   }
   if (rc) return rc;
   if (part) {
