@@ -9,15 +9,16 @@ earlier eager graph of the same leaves may still hold on another stream; take gr
 torch.autograd.grad on leaves of the captured program's own.)  Everything runs on the current stream of the tensors' device; results are
 bit-reproducible."""
 import ctypes
+import functools
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ..lib import current_stream, lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _POS_TYPES = {torch.int64: 0, torch.int32: 1, torch.float32: 2}
 _L2, _L3, _L9, _L15 = (ctypes.c_long * n for n in (2, 3, 9, 15))
+_sections = functools.lru_cache(maxsize=64)(lambda sections: (ctypes.c_int * len(sections))(*sections))   # as the C ABI reads them
 
 
 def _check(what, t0, *tensors):
@@ -43,6 +44,11 @@ def _call(name, device, *args):
     rc = getattr(L.cdll, name)(*args, current_stream(index))
     if rc:
         raise RuntimeError(f"{name} failed ({rc}): {L.cdll.tatt_last_error().decode()}")
+
+
+def _first_order(what):
+    if torch.is_grad_enabled():      # create_graph=True: the gradient would be taken for a constant
+        raise NotImplementedError(f"tatt_amd {what}: no gradient of the gradient")
 
 
 def _ptr(t):
@@ -128,8 +134,8 @@ class _LayerNormFn(torch.autograd.Function):
         return y if residual is None else (y, s)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dsum=None):
+        _first_order("layer_norm")
         s, weight, stat = ctx.saved_tensors
         _, need_r, need_w, need_b, _ = ctx.needs_input_grad
         if dy is None:                                     # only the sum was used
@@ -156,26 +162,27 @@ def rotary_frequencies(sections, base=10000.0, device="cuda"):
 def rotate(q, k, positions, freqs, sections, interleaved=False, inverse=False):
     """`rotary` without autograd; inverse=True turns back (its backward pass)."""
     dtype = _check("rotary", q, k)
-    n = len(sections)
+    n, width = len(sections), sum(sections)
     if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
         raise RuntimeError("tatt_amd rotary: q [B, L, H, D] and k [B, L, Hk, D] expected")
     B, L, H, D = q.shape
-    if not 1 <= n <= 4 or any(s <= 0 or s % 2 for s in sections) or sum(sections) > D:
+    if not 1 <= n <= 4 or min(sections) <= 0 or any(s & 1 for s in sections) or width > D:
         raise RuntimeError(f"tatt_amd rotary: one to four positive even sections of at most {D} dimensions together, got {tuple(sections)}")
-    if positions.dtype not in _POS_TYPES:
+    kind, shape, device = _POS_TYPES.get(positions.dtype), positions.shape, q.device
+    if kind is None:
         raise NotImplementedError(f"tatt_amd rotary: positions are int64, int32 or float32, got {positions.dtype}")
-    if positions.device != q.device or tuple(positions.shape) not in ((L, n), (B, L, n), (1, L, n)):
-        raise RuntimeError(f"tatt_amd rotary: positions [L, axes] or [B, L, axes] on the tensors' device expected, got {tuple(positions.shape)} on {positions.device}")
-    if freqs.dtype != torch.float64 or freqs.shape != (sum(sections) // 2,) or freqs.device != q.device or not freqs.is_contiguous():
+    if positions.device != device or shape[-2:] != (L, n) or len(shape) not in (2, 3) or (len(shape) == 3 and shape[0] not in (1, B)):
+        raise RuntimeError(f"tatt_amd rotary: positions [L, axes] or [B, L, axes] on the tensors' device expected, got {tuple(shape)} on {positions.device}")
+    if freqs.dtype != torch.float64 or freqs.shape != (width // 2,) or freqs.device != device or not freqs.is_contiguous():
         raise RuntimeError("tatt_amd rotary: freqs is a contiguous float64 vector of sum(sections) / 2 on the tensors' device (rotary_frequencies)")
     qo, ko = _like(q), None if k is None else _like(k)
     if qo.numel():
-        q, k = _rows(q), None if k is None or not k.numel() else _rows(k)
+        q, k = _rows(q), None if k is None or not ko.numel() else _rows(k)
         sp = positions.stride()
-        pos_strides = _L3(sp[0] if len(sp) == 3 and positions.shape[0] > 1 else 0, sp[-2], sp[-1])
-        _call("tatt_rotary", q.device, q.data_ptr(), _L3(*q.stride()[:3]), qo.data_ptr(), H, _ptr(k), None if k is None else _L3(*k.stride()[:3]), _ptr(ko),
-              0 if k is None else k.shape[2], positions.data_ptr(), _POS_TYPES[positions.dtype], pos_strides, freqs.data_ptr(),
-              (ctypes.c_int * n)(*sections), n, B, L, D, bool(interleaved), bool(inverse), dtype)
+        pos_strides = _L3(sp[0] if len(sp) == 3 and shape[0] > 1 else 0, sp[-2], sp[-1])
+        _call("tatt_rotary", device, q.data_ptr(), _L3(*q.stride()[:3]), qo.data_ptr(), H, _ptr(k), None if k is None else _L3(*k.stride()[:3]), _ptr(ko),
+              0 if k is None else k.shape[2], positions.data_ptr(), kind, pos_strides, freqs.data_ptr(), _sections(tuple(sections)), n, B, L, D,
+              bool(interleaved), bool(inverse), dtype)
     return qo, ko
 
 
@@ -189,8 +196,8 @@ class _RotaryFn(torch.autograd.Function):
         return qo if k is None else (qo, ko)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dq, dk=None):
+        _first_order("rotary")
         positions, freqs = ctx.saved_tensors
         if dq is None and dk is None:
             return (None,) * 6
@@ -290,8 +297,8 @@ class _AttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
+        _first_order("attention")
         q, k, v, out, lse, mask = ctx.saved_tensors
         return (*attention_backward(dout, q, k, v, out, lse, mask, *ctx.how), None, None, None)
 

@@ -547,3 +547,40 @@ def test_attention_reads_long_sequences_where_they_lie():
     far.copy_(k[:, :40])
     assert T._laid_out(far, 1).data_ptr() != far.data_ptr()
     assert torch.equal(T.attention_forward(q, far, far)[0], T.attention_forward(q, k[:, :40], k[:, :40])[0])
+
+
+def test_no_gradient_of_a_gradient():
+    """Asked for, it is refused: the backward pass is no function that autograd could differentiate."""
+    x = rnd(4, 16, seed=1).requires_grad_()
+    with pytest.raises(NotImplementedError, match="gradient of the gradient"):
+        torch.autograd.grad(T.layer_norm(x).sum(), x, create_graph=True)
+    q = rnd(1, 4, 2, 16, seed=1).requires_grad_()
+    with pytest.raises(NotImplementedError, match="gradient of the gradient"):
+        torch.autograd.grad(T.attention(q, q, q).sum(), q, create_graph=True)
+    with pytest.raises(NotImplementedError, match="gradient of the gradient"):
+        torch.autograd.grad(T.rotary(q, None, torch.zeros(4, 1, dtype=torch.int64, device="cuda"), T.rotary_frequencies((16,)), (16,)).sum(), q, create_graph=True)
+
+
+@pytest.mark.parametrize("what", ["q", "positions", "sections", "freqs", "mask", "residual", "weight", "lse"])
+def test_python_refusals_on_the_gpu(what):
+    """Raised before any launch."""
+    q, at, f = rnd(2, 5, 4, 16, seed=1), torch.zeros(5, 2, dtype=torch.int64, device="cuda"), T.rotary_frequencies((8, 8))
+    x, w = rnd(6, 12, seed=2), torch.ones(12, device="cuda")
+    calls = {
+        "q": [lambda: T.attention(q.half(), q.half(), q.half()), lambda: T.attention(q, q.bfloat16(), q), lambda: T.attention(q, q[:1], q[:1]),
+              lambda: T.attention(q[:, :, :3], q[:, :, :2], q[:, :, :2]), lambda: T.attention(*[rnd(1, 2, 1, 136)] * 3), lambda: T.attention(q, q, q[:, :4]),
+              lambda: T.attention(q[0], q[0], q[0]), lambda: T.attention(q, q.cpu(), q), lambda: T.rotary(q[0], None, at, f, (8, 8))],
+        "positions": [lambda: T.rotary(q, q, at[:4], f, (8, 8)), lambda: T.rotary(q, q, at.double(), f, (8, 8)), lambda: T.rotary(q, q, at.cpu(), f, (8, 8)),
+                      lambda: T.rotary(q, q, at.expand(3, 5, 2), f, (8, 8)), lambda: T.rotary(q, q, at[:, :1], f, (8, 8))],
+        "sections": [lambda: T.rotary(q, q, at, f, (8, 7)), lambda: T.rotary(q, q, at, f, (8, 10)), lambda: T.rotary(q, q, at, f, ()), lambda: T.rotary(q, q, at, f, (16, 0))],
+        "freqs": [lambda: T.rotary(q, q, at, f.float(), (8, 8)), lambda: T.rotary(q, q, at, f[:7], (8, 8)), lambda: T.rotary(q, q, at, f.cpu(), (8, 8))],
+        "mask": [lambda: T.attention(q, q, q, key_padding_mask=torch.zeros(2, 4, dtype=torch.bool, device="cuda")), lambda: T.attention(q, q, q, key_padding_mask=torch.zeros(2, 5, device="cuda")),
+                 lambda: T.attention(q, q, q, key_padding_mask=torch.zeros(2, 5, dtype=torch.bool))],
+        "residual": [lambda: T.layer_norm(x, residual=x[:5]), lambda: T.layer_norm(x, residual=x.bfloat16()), lambda: T.layer_norm(x[:, :0])],
+        "weight": [lambda: T.layer_norm(x, w[:11]), lambda: T.layer_norm(x, w.bfloat16()), lambda: T.layer_norm(x, w, w.cpu()), lambda: T.layer_norm(x.double())],
+        "lse": [lambda: T.attention_backward(q, q, q, q, q, torch.zeros(2, 4, 4, device="cuda")), lambda: T.attention_backward(q[:, :4], q, q, q, q, torch.zeros(2, 4, 5, device="cuda")),
+                lambda: T.layer_norm_backward(x, x, w, torch.zeros(5, 2, device="cuda"))],
+    }
+    for call in calls[what]:
+        with pytest.raises((RuntimeError, NotImplementedError), match="tatt_amd"):
+            call()
