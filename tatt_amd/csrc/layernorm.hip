@@ -19,17 +19,17 @@ struct Row {
 #pragma unroll
     for (int n = 0; n < NV; ++n) c[n] = load_chunk<T>(row, n * TPR + t, C, vec);
   }
-  __device__ __forceinline__ void get(int n, float (&f)[Elem<T>::PER_CHUNK]) const {
-    T e[Elem<T>::PER_CHUNK];
+  __device__ __forceinline__ void get(int n, float (&f)[per_chunk<T>()]) const {
+    T e[per_chunk<T>()];
     memcpy(e, &c[n], 16);
 #pragma unroll
-    for (int i = 0; i < Elem<T>::PER_CHUNK; ++i) f[i] = to_f32(e[i]);
+    for (int i = 0; i < per_chunk<T>(); ++i) f[i] = to_f32(e[i]);
   }
 };
 
 // chunk c of a row from floats, rounded to T
 template <typename T>
-__device__ __forceinline__ uint4 round_chunk(const float (&f)[Elem<T>::PER_CHUNK]) {
+__device__ __forceinline__ uint4 round_chunk(const float (&f)[per_chunk<T>()]) {
   uint4 u;
   if constexpr (sizeof(T) == 4) {
     u = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
@@ -42,7 +42,7 @@ __device__ __forceinline__ uint4 round_chunk(const float (&f)[Elem<T>::PER_CHUNK
 
 template <typename T>
 __device__ __forceinline__ void store_chunk(T* row, int c, int C, int vec, uint4 u) {
-  constexpr int E = Elem<T>::PER_CHUNK;
+  constexpr int E = per_chunk<T>();
   if (vec) {
     if (c * E < C) *reinterpret_cast<uint4*>(row + c * E) = u;
   } else {
@@ -98,7 +98,7 @@ template <typename T, int TPR, int NV, int vec>
 __global__ __launch_bounds__(block_of(TPR)) void layernorm_fwd_kernel(const T* __restrict__ x, long ldx, const T* __restrict__ res, long ldr,
                                                             const float* __restrict__ gamma, const float* __restrict__ beta, T* __restrict__ sum,
                                                             T* __restrict__ y, float* __restrict__ stat, long rows, int C, float eps) {
-  constexpr int E = Elem<T>::PER_CHUNK, PER = block_of(TPR) / TPR;
+  constexpr int E = per_chunk<T>(), PER = block_of(TPR) / TPR;
   __shared__ float red[32];
   const int t = threadIdx.x % TPR;
   for (long r0 = (long)blockIdx.x * PER; r0 < rows; r0 += (long)gridDim.x * PER) {
@@ -159,7 +159,7 @@ template <typename T, int TPR, int NV, int vec, bool PARAMS>
 __global__ __launch_bounds__(block_of(TPR)) void layernorm_bwd_kernel(const T* __restrict__ s, long lds, const T* __restrict__ dy, long lddy, const T* __restrict__ dsum,
                                                             long ldds, const float* __restrict__ gamma, const float* __restrict__ stat,
                                                             T* __restrict__ dx, float* __restrict__ partial, long rows, int C) {
-  constexpr int E = Elem<T>::PER_CHUNK, PER = block_of(TPR) / TPR;
+  constexpr int E = per_chunk<T>(), PER = block_of(TPR) / TPR;
   __shared__ float red[32];
   __shared__ float cols[PARAMS && PER > 1 ? 256 * E : 1];  // one chunk of every thread at a time
   const int t = threadIdx.x % TPR;

@@ -14,8 +14,8 @@
 //   dimensions x contraction over the tile's rows         (O, dQ, dK, dV)       A = the tile transposed
 // The accumulator of the first kind (lane = column, registers = tile rows 8 (i / 4) + 4 half + i % 4) is, register for register, a B operand of
 // the second kind if the contraction visits the tile's rows in that order: no element changes its lane between the two products.
-//   bf16: v_mfma_f32_32x32x16_bf16, a chunk pair (16 dimensions) a step; transposed reads are ds_read_b64_tr_b16 (4 rows x 16 dimensions to 16 lanes)
-//   fp32: v_mfma_f32_32x32x2_f32, four a step (8 dimensions); transposed reads are 4-byte reads along a row
+// The MFMA is v_mfma_f32_32x32x16_bf16; transposed reads are ds_read_b64_tr_b16 (4 rows x 16 dimensions to 16 lanes).  fp32 tensors go through the
+// same products as three bf16 pieces of every operand (fp32 accuracy; 6 bf16 MFMAs of 8 passes against 8 fp32 ones of 16).
 // Operands are rounded to bf16 only where the tensors are bf16 (P and dS enter their second product in bf16: 2^-9 of a term, the error that the
 // stored result carries anyway); accumulation is fp32.
 #pragma once
@@ -23,25 +23,74 @@
 
 namespace {
 
-__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x16 mma(f32x4 a, f32x4 b, f32x16 c) {
-#pragma unroll
-  for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[t], b[t], c, 0, 0, 0);
-  return c;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// A lane's 8 contraction places of a step, as the matrix core takes them.  bf16 tensors: the values.  fp32 tensors: three bf16 pieces of each value,
+// x = x0 + x1 + x2 exactly (3 x 8 significant bits); a product is the six terms a0 b0 + (a0 b1 + a1 b0) + (a0 b2 + a1 b1 + a2 b0), added in fp32,
+// smallest first, and what is left out is below the rounding of one fp32 product.
+template <typename T>
+struct Frag {
+  static constexpr int PIECES = sizeof(T) == 2 ? 1 : 3;
+  bf16x8 p[PIECES];
+};
+
+template <typename T>
+__device__ __forceinline__ f32x16 mma(const Frag<T>& a, const Frag<T>& b, f32x16 c) {
+  if constexpr (Frag<T>::PIECES == 3) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[2], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[2], b.p[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[0], c, 0, 0, 0);
+  }
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], c, 0, 0, 0);
 }
 
-// accumulator registers [step * n, step * n + n) as the B operand of the transposed product's step (n = 8 bf16, 4 fp32); bf16: rounded to nearest even
-template <typename T>
-__device__ __forceinline__ typename Elem<T>::Frag pack_step(const f32x16& c, int step) {
-  typename Elem<T>::Frag r;
+// two values as bf16 (nearest even), low half first; and the values that it stands for
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  const b2 v = __builtin_convertvector((f2{a, b}), b2);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float low2(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float high2(uint32_t u) { return __uint_as_float(u & 0xFFFF0000u); }
+
+// two fp32 values as three pieces each (of an infinity the remainder is no number: what it reaches is NaN)
+__device__ __forceinline__ void split2(float a, float b, uint32_t (&u)[3]) {
+  u[0] = pack2(a, b);
+  const float ra = a - low2(u[0]), rb = b - high2(u[0]);
+  u[1] = pack2(ra, rb);
+  u[2] = pack2(ra - low2(u[1]), rb - high2(u[1]));
+}
+
+// 8 values, v(0) .. v(7), as a fragment
+template <typename T, typename V>
+__device__ __forceinline__ Frag<T> fragment(V v) {
+  uint32_t u[Frag<T>::PIECES][4];
 #pragma unroll
-  for (int j = 0; j < Elem<T>::PER_CHUNK; ++j) {
-    if constexpr (sizeof(T) == 4)
-      r[j] = c[step * 4 + j];
-    else
-      r[j] = (__bf16)c[step * 8 + j];
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (Frag<T>::PIECES == 3) {
+      uint32_t w[3];
+      split2(v(2 * j), v(2 * j + 1), w);
+#pragma unroll
+      for (int x = 0; x < 3; ++x) u[x][j] = w[x];
+    } else {
+      u[0][j] = pack2(v(2 * j), v(2 * j + 1));
+    }
   }
-  return r;
+  Frag<T> f;
+  memcpy(&f, u, sizeof(f));
+  return f;
+}
+
+constexpr int STEP = 16;  // contraction places of an MFMA step (both lane halves)
+
+// accumulator registers 8 step .. 8 step + 7 as the B operand of the transposed product's step
+template <typename T>
+__device__ __forceinline__ Frag<T> pack_step(const f32x16& c, int step) {
+  return fragment<T>([&](int j) { return c[8 * step + j]; });
 }
 
 // waves a SIMD that the registers are shared out for.  Two (256 registers each) unless what a wave has to hold -- the fragments of its rows, the
@@ -56,66 +105,70 @@ constexpr int dkv_waves(int DK) { return DK > 64 || (sizeof(T) == 4 && DK == 64)
 // head widths the kernels are built for, and the LDS row that holds one
 constexpr int row_width(int DK) { return DK <= 32 ? 32 : DK <= 64 ? 64 : 128; }
 
-// A row-major LDS tile of W elements a row (a power of two, 32 to 128).  The 16-byte chunks of row r are stored at chunk ^ swizzle(r): the 16
-// rows of a chunk column fall into 16 different 16-byte slots of the 256 bytes that LDS serves at once, and so do the chunks that four
-// neighbouring rows of a transposed read take.
-template <typename T, int W>
+// A row-major LDS tile of ROWS rows of W bf16 elements (W a power of two, 32 to 128), or three such planes, one for each piece.  The 16-byte chunks
+// of row r are stored at chunk ^ swizzle(r): the 16 rows of a chunk column fall into 16 different 16-byte slots of the 256 bytes that LDS serves at
+// once, and so do the chunks that four neighbouring rows of a transposed read take (no bank conflict is counted).
+template <typename T, int W, int ROWS>
 struct Tile {
-  static constexpr int NC = W * (int)sizeof(T) / 16;  // chunks of a row: 4, 8, 16 or 32
-  static constexpr int ROW = NC * 16;                 // bytes of a row
+  static constexpr int NC = W / 8;    // chunks of a row: 4, 8 or 16
+  static constexpr int ROW = W * 2;   // bytes of a row
+  static constexpr int PLANE = ROWS * ROW, BYTES = PLANE * Frag<T>::PIECES;
   __device__ __forceinline__ static int swizzle(int r) {
-    if (NC >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+    if (NC == 16) return ((r & 3) << 2) | ((r >> 2) & 3);
     if (NC == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
     return (r >> 2) & 3;
   }
   __device__ __forceinline__ static int offset(int r, int chunk) { return r * ROW + ((chunk ^ swizzle(r)) << 4); }
 
+  // 16 bytes of a row of the tensor, its chunk c (8 bf16 or 4 fp32 elements), into the tile
+  __device__ __forceinline__ static void put(char* tile, int r, int c, uint4 v) {
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint4*>(tile + offset(r, c)) = v;
+    } else {
+      uint32_t a[3], b[3];
+      split2(__uint_as_float(v.x), __uint_as_float(v.y), a);
+      split2(__uint_as_float(v.z), __uint_as_float(v.w), b);
+#pragma unroll
+      for (int x = 0; x < 3; ++x) *reinterpret_cast<uint2*>(tile + x * PLANE + offset(r, c >> 1) + 8 * (c & 1)) = make_uint2(a[x], b[x]);
+    }
+  }
+
   // Where a lane reads: (its base ^ a constant) + a constant, so one register serves every fragment of a kind.
   struct Lane {
     int row, col;
     __device__ __forceinline__ explicit Lane(int lane) {
-      const int half = lane >> 5;
+      const int half = lane >> 5, i = lane & 15, piece = i & 3;
       row = offset(lane & 31, half);
-      if constexpr (sizeof(T) == 4) {
-        const int d = lane & 31;
-        col = 4 * half * ROW + (((d >> 2) ^ half) << 4) + 4 * (d & 3);
-      } else {  // 16 lanes read four rows x 32 bytes (lane i: row i / 4, 8-byte piece i % 4) and receive column lane % 16 of those four rows
-        const int i = lane & 15, piece = i & 3;
-        col = offset(4 * half + (i >> 2), 2 * ((lane >> 4) & 1) + (piece >> 1)) + 8 * (piece & 1);
-      }
+      // 16 lanes read four rows x 32 bytes (lane i: row i / 4, 8-byte piece i % 4) and receive column lane % 16 of those four rows
+      col = offset(4 * half + (i >> 2), 2 * ((lane >> 4) & 1) + (piece >> 1)) + 8 * (piece & 1);
     }
     // keeps the compiler from holding each base ^ constant in a register of its own across the loop (and spilling them)
     __device__ __forceinline__ void afresh() { asm volatile("" : "+v"(row), "+v"(col)); }
   };
 
   // A operand of a row product: lane (row = lane % 32, half) holds chunk 2 step + half of its row.  row0 a multiple of 32.
-  __device__ __forceinline__ static typename Elem<T>::Frag rows(const char* tile, int row0, int step, const Lane& at) {
-    return *reinterpret_cast<const typename Elem<T>::Frag*>(tile + row0 * ROW + (at.row ^ (step << 5)));
+  __device__ __forceinline__ static Frag<T> rows(const char* tile, int row0, int step, const Lane& at) {
+    Frag<T> f;
+#pragma unroll
+    for (int x = 0; x < Frag<T>::PIECES; ++x) f.p[x] = *reinterpret_cast<const bf16x8*>(tile + x * PLANE + row0 * ROW + (at.row ^ (step << 5)));
+    return f;
   }
 
   // A operand of a transposed product: lane (dimension d0 + lane % 32, half) holds the tile rows that accumulator registers of `step` stand for:
-  // fp32: row0 + 8 step + 4 half + j;  bf16: row0 + 16 step + 4 half + {0..3, 8..11}.  d0 and row0 multiples of 32.
-  __device__ __forceinline__ static typename Elem<T>::Frag transposed(const char* tile, int row0, int step, int d0, const Lane& at) {
-    if constexpr (sizeof(T) == 4) {
-      f32x4 r;
+  // row0 + 16 step + 4 half + {0..3, 8..11}.  d0 and row0 multiples of 32.
+  __device__ __forceinline__ static Frag<T> transposed(const char* tile, int row0, int step, int d0, const Lane& at) {
+    union {
+      s16x4 q[Frag<T>::PIECES][2];
+      Frag<T> f;
+    } u;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int turn = (NC >= 16 ? j << 2 : (j >> 1) << 2) ^ (2 * (step & 1)) ^ (d0 >> 2);  // swizzle of row 8 step + 4 half + j, and the chunk of d0
-        r[j] = *reinterpret_cast<const float*>(tile + (row0 + 8 * step + j) * ROW + (at.col ^ (turn << 4)));
-      }
-      return r;
-    } else {
-      union {
-        s16x4 q[2];
-        bf16x8 f;
-      } u;
+    for (int x = 0; x < Frag<T>::PIECES; ++x)
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const char* p = tile + (row0 + 16 * step + 8 * s) * ROW + (at.col ^ (((d0 >> 3) ^ (2 * s)) << 4));
-        u.q[s] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+        const char* p = tile + x * PLANE + (row0 + 16 * step + 8 * s) * ROW + (at.col ^ (((d0 >> 3) ^ (2 * s)) << 4));
+        u.q[x][s] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
       }
-      return u.f;
-    }
+    return u.f;
   }
 };
 
@@ -162,17 +215,48 @@ __device__ __forceinline__ long row_offset(int r, int G, long sl, long sh) {
 // B operand of a row product: this lane's row, all steps of the contraction
 template <typename T, int DK>
 struct RowFrags {
-  typename Elem<T>::Frag f[DK / Elem<T>::STEP];
+  Frag<T> f[DK / STEP];
   __device__ __forceinline__ void load(const T* row, bool on, int D, int lane) {
 #pragma unroll
-    for (int s = 0; s < DK / Elem<T>::STEP; ++s) {
-      const uint4 u = on ? load_chunk<T>(row, 2 * s + (lane >> 5), D, 1) : make_uint4(0, 0, 0, 0);
-      memcpy(&f[s], &u, 16);
+    for (int s = 0; s < DK / STEP; ++s) {
+      T t[8];
+      chunk8(row, on, s, D, lane, t);
+      if constexpr (sizeof(T) == 2)
+        memcpy(&f[s], t, 16);
+      else
+        f[s] = fragment<T>([&](int j) { return t[j]; });
     }
+  }
+  // the product with another row
+  __device__ __forceinline__ float dot(const T* row, bool on, int D, int lane) const {
+    float d = 0.f;
+#pragma unroll
+    for (int s = 0; s < DK / STEP; ++s) {
+      T t[8];
+      chunk8(row, on, s, D, lane, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float v = 0.f;
+#pragma unroll
+        for (int x = Frag<T>::PIECES - 1; x >= 0; --x) v += (float)f[s].p[x][j];
+        d += to_f32(t[j]) * v;
+      }
+    }
+    return d;
   }
   __device__ __forceinline__ void negate() {
 #pragma unroll
-    for (int s = 0; s < DK / Elem<T>::STEP; ++s) f[s] = -f[s];
+    for (int s = 0; s < DK / STEP; ++s)
+#pragma unroll
+      for (int x = 0; x < Frag<T>::PIECES; ++x) f[s].p[x] = -f[s].p[x];
+  }
+  // elements 16 s + 8 half .. + 7 of a row
+  __device__ __forceinline__ static void chunk8(const T* row, bool on, int s, int D, int lane, T (&t)[8]) {
+    constexpr int N = 8 / per_chunk<T>();
+    uint4 u[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) u[n] = on ? load_chunk<T>(row, (2 * s + (lane >> 5)) * N + n, D, 1) : make_uint4(0, 0, 0, 0);
+    memcpy(t, u, 8 * sizeof(T));
   }
 };
 
@@ -181,7 +265,7 @@ struct RowFrags {
 // for which the load returns zeros.  LINEAR: rows are one stride apart (keys), else at places(r) (queries of several heads).
 template <typename T, int W, int ROWS, int NT, bool LINEAR>
 struct Stage {
-  static constexpr int NC = Tile<T, W>::NC, N = (ROWS * NC + NT - 1) / NT, STEP = NT / NC;
+  static constexpr int NC = W / per_chunk<T>(), N = (ROWS * NC + NT - 1) / NT, HOP = NT / NC;
   static_assert(NT % NC == 0 && (N == 1 || ROWS * NC % NT == 0), "every thread holds the same chunk of N rows");
   static constexpr int NOWHERE = 0x7FFFFFF0;
   typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -189,18 +273,18 @@ struct Stage {
   int off[LINEAR ? 1 : N];  // byte offsets from the tile's first row
   int hop;                  // LINEAR: bytes between a thread's rows
 
-  __device__ __forceinline__ static int row(int n) { return n * STEP + (int)threadIdx.x / NC; }
+  __device__ __forceinline__ static int row(int n) { return n * HOP + (int)threadIdx.x / NC; }
   __device__ __forceinline__ static int chunk() { return (int)threadIdx.x % NC; }
 
   __device__ __forceinline__ void linear(long stride, int D) {
     static_assert(LINEAR, "");
-    off[0] = chunk() * Elem<T>::PER_CHUNK < D && row(0) < ROWS ? (int)(row(0) * stride * (long)sizeof(T)) + chunk() * 16 : NOWHERE;
-    hop = (int)(STEP * stride * (long)sizeof(T));
+    off[0] = chunk() * per_chunk<T>() < D && row(0) < ROWS ? (int)(row(0) * stride * (long)sizeof(T)) + chunk() * 16 : NOWHERE;
+    hop = (int)(HOP * stride * (long)sizeof(T));
   }
   template <typename Offset>
   __device__ __forceinline__ void places(Offset offset, int D) {
     static_assert(!LINEAR, "");
-    const bool on = chunk() * Elem<T>::PER_CHUNK < D && row(0) < ROWS;
+    const bool on = chunk() * per_chunk<T>() < D && row(0) < ROWS;
 #pragma unroll
     for (int n = 0; n < N; ++n) off[n] = on ? (int)(offset(row(n)) * (long)sizeof(T)) + chunk() * 16 : NOWHERE;
   }
@@ -219,7 +303,7 @@ struct Stage {
   __device__ __forceinline__ void put(char* tile) const {
     if (row(0) >= ROWS) return;
 #pragma unroll
-    for (int n = 0; n < N; ++n) *reinterpret_cast<i32x4*>(tile + Tile<T, W>::offset(row(n), chunk())) = r[n];
+    for (int n = 0; n < N; ++n) Tile<T, W, ROWS>::put(tile, row(n), chunk(), make_uint4(r[n][0], r[n][1], r[n][2], r[n][3]));
   }
   // zeros in the rows whose bit is not set
   template <int NW>
@@ -406,11 +490,9 @@ int prepare_launch(const MhaArgs& a, K kernel, int threads, size_t bytes) {
   return TATT_OK;
 }
 
-template <typename T, int DK>
-struct Shape {
-  static constexpr int W = row_width(DK), ROW = Tile<T, W>::ROW;
-  static constexpr int WK = ROW > 256 ? 2 : 4;  // waves along the summed axis: two tiles of 32 WK rows within 64 KB
-};
+// waves along the summed axis where the other axis has one tile: two tiles of 32 of their rows within 64 KB
+template <typename T>
+constexpr int narrow_waves(int DK) { return sizeof(T) == 2 ? (DK > 64 ? 2 : 4) : (DK > 64 ? 1 : DK > 32 ? 2 : 4); }
 
 }  // namespace
 

@@ -8,8 +8,8 @@ namespace {
 // dQ and delta.  WQ waves of 32 R rows; registers hold Q and dO, LDS tiles of 32 SUB keys K and V.
 template <typename T, int DK, int WQ, int R, int SUB>
 __global__ __launch_bounds__(64 * WQ, dq_waves<T>(DK)) void mha_dq_kernel(MhaArgs a, T* __restrict__ dq, float* __restrict__ part) {
-  constexpr int NT = 64 * WQ, W = row_width(DK), ND = (DK + 31) / 32, KT = 32 * SUB, TILE = KT * Tile<T, W>::ROW;
-  constexpr int NS = DK / Elem<T>::STEP, TS = 32 / Elem<T>::STEP, NB = 4 * TILE <= 64 * 1024 ? 2 : 1;
+  constexpr int NT = 64 * WQ, W = row_width(DK), ND = (DK + 31) / 32, KT = 32 * SUB, TILE = Tile<T, W, KT>::BYTES;
+  constexpr int NS = DK / STEP, TS = 32 / STEP, NB = 4 * TILE <= 64 * 1024 ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wq = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const Where w = where(a);
@@ -36,15 +36,7 @@ __global__ __launch_bounds__(64 * WQ, dq_waves<T>(DK)) void mha_dq_kernel(MhaArg
     gf[r].load((const T*)a.dout + w.b * a.dos[0] + query[r] * a.dos[1] + h * a.dos[2], on, a.D, lane);
     if (a.scale < 0.f) qf[r].negate();
     const T* orow = (const T*)a.out + w.b * a.os[0] + query[r] * a.os[1] + h * a.os[2];
-    float d = 0.f;
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const uint4 u = load_chunk<T>(orow, 2 * s + half, a.D, 1);
-      T t[Elem<T>::PER_CHUNK];
-      memcpy(t, &u, 16);
-#pragma unroll
-      for (int e = 0; e < Elem<T>::PER_CHUNK; ++e) d += to_f32(t[e]) * (float)gf[r].f[s][e];
-    }
+    const float d = gf[r].dot(orow, on, a.D, lane);
     const long stat = (w.b * a.H + h) * a.Lq + query[r];
     lse[r] = on ? a.lse[stat] : INFINITY;
     delta[r] = lse[r] == INFINITY ? 0.f : half_sum(d);  // a row that sees nothing: whatever dO holds there
@@ -72,7 +64,7 @@ __global__ __launch_bounds__(64 * WQ, dq_waves<T>(DK)) void mha_dq_kernel(MhaArg
     vs.put(to + TILE);
     now = next;
   };
-  typename Tile<T, W>::Lane place(lane);
+  typename Tile<T, W, KT>::Lane place(lane);
   int at = 0;
   if (kbeg < kend) {
     fetch(kbeg);
@@ -95,13 +87,13 @@ __global__ __launch_bounds__(64 * WQ, dq_waves<T>(DK)) void mha_dq_kernel(MhaArg
       }
 #pragma unroll
       for (int t = 0; t < NS; ++t) {
-        const auto k = Tile<T, W>::rows(kt, 32 * s, t, place);
+        const auto k = Tile<T, W, KT>::rows(kt, 32 * s, t, place);
 #pragma unroll
         for (int r = 0; r < R; ++r) sc[r] = mma(k, qf[r].f[t], sc[r]);
       }
 #pragma unroll
       for (int t = 0; t < NS; ++t) {
-        const auto v = Tile<T, W>::rows(vt, 32 * s, t, place);
+        const auto v = Tile<T, W, KT>::rows(vt, 32 * s, t, place);
 #pragma unroll
         for (int r = 0; r < R; ++r) dp[r] = mma(v, gf[r].f[t], dp[r]);
       }
@@ -117,7 +109,7 @@ __global__ __launch_bounds__(64 * WQ, dq_waves<T>(DK)) void mha_dq_kernel(MhaArg
           for (int i = 0; i < 16; ++i) sc[r][i] = see >> acc_row(i) & 1 ? sc[r][i] : 0.f;
         }
       }
-      typename Elem<T>::Frag p[R][TS];
+      Frag<T> p[R][TS];
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -126,7 +118,7 @@ __global__ __launch_bounds__(64 * WQ, dq_waves<T>(DK)) void mha_dq_kernel(MhaArg
       for (int t = 0; t < TS; ++t)
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt) {
-          const auto k = Tile<T, W>::transposed(kt, 32 * s, t, 32 * dt, place);
+          const auto k = Tile<T, W, KT>::transposed(kt, 32 * s, t, 32 * dt, place);
 #pragma unroll
           for (int r = 0; r < R; ++r) o[r][dt] = mma(k, p[r][t], o[r][dt]);
         }
@@ -153,8 +145,8 @@ __global__ __launch_bounds__(64 * WQ, dq_waves<T>(DK)) void mha_dq_kernel(MhaArg
 // dK and dV.  WN waves along the keys (32 each) x WR along the rows; LDS holds tiles of 32 WR SUB rows of Q and dO, and their lse and delta.
 template <typename T, int DK, int WN, int WR, int SUB>
 __global__ __launch_bounds__(64 * WN * WR, dkv_waves<T>(DK)) void mha_dkv_kernel(MhaArgs a, T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part) {
-  constexpr int NT = 64 * WN * WR, W = row_width(DK), ND = (DK + 31) / 32, RT = 32 * WR * SUB, TILE = RT * Tile<T, W>::ROW, BUF = 2 * TILE + 2 * RT * 4;
-  constexpr int NS = DK / Elem<T>::STEP, TS = 32 / Elem<T>::STEP, NB = 4 * TILE <= 64 * 1024 ? 2 : 1;
+  constexpr int NT = 64 * WN * WR, W = row_width(DK), ND = (DK + 31) / 32, RT = 32 * WR * SUB, TILE = Tile<T, W, RT>::BYTES, BUF = 2 * TILE + 2 * RT * 4;
+  constexpr int NS = DK / STEP, TS = 32 / STEP, NB = 4 * TILE <= 64 * 1024 ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wr = wave / WN, half = lane >> 5;
   const Where w = where(a);
@@ -212,7 +204,7 @@ __global__ __launch_bounds__(64 * WN * WR, dkv_waves<T>(DK)) void mha_dkv_kernel
     float* ls = reinterpret_cast<float*>(to + 2 * TILE);
     if (threadIdx.x < RT) ls[threadIdx.x] = l0, ls[RT + threadIdx.x] = d0;
   };
-  typename Tile<T, W>::Lane place(lane);
+  typename Tile<T, W, RT>::Lane place(lane);
   if (any && rbeg < rend) {
     int buf = 0;
     if (steady) places(0);
@@ -233,9 +225,9 @@ __global__ __launch_bounds__(64 * WN * WR, dkv_waves<T>(DK)) void mha_dkv_kernel
         clear(sc);
         clear(dp);
 #pragma unroll
-        for (int t = 0; t < NS; ++t) sc = mma(Tile<T, W>::rows(qt, at, t, place), kf.f[t], sc);
+        for (int t = 0; t < NS; ++t) sc = mma(Tile<T, W, RT>::rows(qt, at, t, place), kf.f[t], sc);
 #pragma unroll
-        for (int t = 0; t < NS; ++t) dp = mma(Tile<T, W>::rows(gt, at, t, place), vf.f[t], dp);
+        for (int t = 0; t < NS; ++t) dp = mma(Tile<T, W, RT>::rows(gt, at, t, place), vf.f[t], dp);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const f32x4 lq = *reinterpret_cast<const f32x4*>(ls + at + 8 * q + 4 * half);
@@ -257,13 +249,13 @@ __global__ __launch_bounds__(64 * WN * WR, dkv_waves<T>(DK)) void mha_dkv_kernel
         for (int t = 0; t < TS; ++t) {
           const auto p = pack_step<T>(sc, t);
 #pragma unroll
-          for (int dt = 0; dt < ND; ++dt) ov[dt] = mma(Tile<T, W>::transposed(gt, at, t, 32 * dt, place), p, ov[dt]);
+          for (int dt = 0; dt < ND; ++dt) ov[dt] = mma(Tile<T, W, RT>::transposed(gt, at, t, 32 * dt, place), p, ov[dt]);
         }
 #pragma unroll
         for (int t = 0; t < TS; ++t) {
           const auto p = pack_step<T>(dp, t);
 #pragma unroll
-          for (int dt = 0; dt < ND; ++dt) ok[dt] = mma(Tile<T, W>::transposed(qt, at, t, 32 * dt, place), p, ok[dt]);
+          for (int dt = 0; dt < ND; ++dt) ok[dt] = mma(Tile<T, W, RT>::transposed(qt, at, t, 32 * dt, place), p, ok[dt]);
         }
       }
       if (r0 + RT < rend) {
@@ -325,7 +317,7 @@ Plan plan_dkv(int B, int Lq, int Lk, int H, int Hkv) { return plan((long)B * Hkv
 
 template <typename T, int DK, int R, int SUB>
 int launch_dq(const MhaArgs& a, T* dq, float* part, hipStream_t st) {
-  const size_t tiles = 2 * 32 * SUB * Shape<T, DK>::ROW, lds = 2 * tiles <= 64 * 1024 ? 2 * tiles : tiles;
+  const size_t tiles = 2 * Tile<T, row_width(DK), 32 * SUB>::BYTES, lds = 2 * tiles <= 64 * 1024 ? 2 * tiles : tiles;
   const auto kernel = mha_dq_kernel<T, DK, 4, R, SUB>;
   if (int rc = prepare_launch(a, kernel, 256, lds)) return rc;
   hipLaunchKernelGGL(kernel, dim3((unsigned)((long)a.B * a.Hkv * a.nblk * a.nsplit)), dim3(256), lds, st, a, dq, part);
@@ -335,8 +327,7 @@ int launch_dq(const MhaArgs& a, T* dq, float* part, hipStream_t st) {
 
 template <typename T, int DK, int WN, int WR, int SUB>
 int launch_dkv(const MhaArgs& a, T* dk, T* dv, float* part, hipStream_t st) {
-  using S = Shape<T, DK>;
-  const size_t tiles = 2 * 32 * WR * SUB * S::ROW, buf = tiles + 2 * 32 * WR * SUB * 4, join = WR > 1 ? (size_t)WN * 32 * (S::W + 4) * 4 : 0;
+  const size_t tiles = 2 * Tile<T, row_width(DK), 32 * WR * SUB>::BYTES, buf = tiles + 2 * 32 * WR * SUB * 4, join = WR > 1 ? (size_t)WN * 32 * (row_width(DK) + 4) * 4 : 0;
   size_t lds = 2 * tiles <= 64 * 1024 ? 2 * buf : buf;
   if (join > lds) lds = join;
   if (int rc = prepare_launch(a, mha_dkv_kernel<T, DK, WN, WR, SUB>, 64 * WN * WR, lds)) return rc;
@@ -347,15 +338,16 @@ int launch_dkv(const MhaArgs& a, T* dk, T* dv, float* part, hipStream_t st) {
 
 template <typename T, int DK>
 int run_bwd(MhaArgs& a, T* dq, T* dk, T* dv, float* part, hipStream_t st) {
-  using S = Shape<T, DK>;
   Plan p = plan_dq(a.B, a.Lq, a.Lk, a.H, a.Hkv);
   a.nsplit = p.nsplit, a.per_split = p.per_split;
   float* q_part = a.nsplit > 1 ? part : nullptr;
-  int rc;
-  if (sizeof(T) == 2 && DK <= 64 && (long)a.B * a.Hkv * a.nsplit * cdiv(a.rows, 256) >= 256) {
-    a.nblk = cdiv(a.rows, 256);
-    rc = launch_dq<T, DK, (sizeof(T) == 2 && DK <= 64 ? 2 : 1), 2>(a, dq, q_part, st);
-  } else {
+  int rc = -1;
+  if constexpr (sizeof(T) == 2 && DK <= 64)
+    if ((long)a.B * a.Hkv * a.nsplit * cdiv(a.rows, 256) >= 256) {
+      a.nblk = cdiv(a.rows, 256);
+      rc = launch_dq<T, DK, 2, 2>(a, dq, q_part, st);
+    }
+  if (rc < 0) {
     a.nblk = cdiv(a.rows, 128);
     rc = launch_dq<T, DK, 1, (DK > 64 && sizeof(T) == 4 ? 1 : 2)>(a, dq, q_part, st);
   }
@@ -368,7 +360,7 @@ int run_bwd(MhaArgs& a, T* dq, T* dk, T* dv, float* part, hipStream_t st) {
   p = plan_dkv(a.B, a.Lq, a.Lk, a.H, a.Hkv);
   a.nblk = p.nblk, a.nsplit = p.nsplit, a.per_split = p.per_split;
   float* kv_part = a.nsplit > 1 ? part : nullptr;
-  if ((rc = p.wide ? launch_dkv<T, DK, 4, 1, (sizeof(T) == 4 ? 1 : DK > 64 ? 2 : 4)>(a, dk, dv, kv_part, st) : launch_dkv<T, DK, 1, S::WK, 1>(a, dk, dv, kv_part, st))) return rc;
+  if ((rc = p.wide ? launch_dkv<T, DK, 4, 1, (sizeof(T) == 4 ? 1 : DK > 64 ? 2 : 4)>(a, dk, dv, kv_part, st) : launch_dkv<T, DK, 1, narrow_waves<T>(DK), 1>(a, dk, dv, kv_part, st))) return rc;
   if (kv_part) {
     const long n = (long)a.B * a.Hkv * a.Lk * a.D;
     hipLaunchKernelGGL(mha_sum_kernel<T>, dim3(cdiv(2 * n, 256)), dim3(256), 0, st, part, a.nsplit, n, dk, dv);

@@ -10,8 +10,8 @@ constexpr float LAZY = 8.f;       // the running maximum follows only rises of m
 // WQ waves along the rows (32 R each) x WK along the keys; tiles of 32 SUB keys for a wave, JOINT of them sharing a look at the maximum.
 template <typename T, int DK, int WQ, int R, int WK, int SUB, int JOINT>
 __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel(MhaArgs a, T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part) {
-  constexpr int NT = 64 * WQ * WK, W = row_width(DK), ND = (DK + 31) / 32, KT = 32 * WK * SUB, TILE = KT * Tile<T, W>::ROW;
-  constexpr int NS = DK / Elem<T>::STEP, TS = 32 / Elem<T>::STEP, NB = 4 * TILE <= 64 * 1024 ? 2 : 1;
+  constexpr int NT = 64 * WQ * WK, W = row_width(DK), ND = (DK + 31) / 32, KT = 32 * WK * SUB, TILE = Tile<T, W, KT>::BYTES;
+  constexpr int NS = DK / STEP, TS = 32 / STEP, NB = 4 * TILE <= 64 * 1024 ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wq = wave % WQ, wk = wave / WQ, half = lane >> 5;
   const Where w = where(a);
@@ -46,7 +46,7 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
   KeyBits<KT> next, now;
   ks.linear(a.ks[1], a.D);
   vs.linear(a.vs[1], a.D);
-  typename Tile<T, W>::Lane place(lane);
+  typename Tile<T, W, KT>::Lane place(lane);
   auto fetch = [&](int k0) {
     ks.load(kb + k0 * a.ks[1], 0, kend - k0);
     vs.load(vb + k0 * a.vs[1], 0, kend - k0);
@@ -83,7 +83,7 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
         for (int r = 0; r < R; ++r) clear(sc[s][r]);
 #pragma unroll
         for (int t = 0; t < NS; ++t) {
-          const auto k = Tile<T, W>::rows(kt, j0 + 32 * s, t, place);
+          const auto k = Tile<T, W, KT>::rows(kt, j0 + 32 * s, t, place);
 #pragma unroll
           for (int r = 0; r < R; ++r) sc[s][r] = mma(k, qf[r].f[t], sc[s][r]);
         }
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
       }
 #pragma unroll
       for (int s = 0; s < JOINT; ++s) {
-        typename Elem<T>::Frag p[R][TS];
+        Frag<T> p[R][TS];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
 #pragma unroll
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
         for (int t = 0; t < TS; ++t)
 #pragma unroll
           for (int dt = 0; dt < ND; ++dt) {
-            const auto v = Tile<T, W>::transposed(vt, j0 + 32 * s, t, 32 * dt, place);
+            const auto v = Tile<T, W, KT>::transposed(vt, j0 + 32 * s, t, 32 * dt, place);
 #pragma unroll
             for (int r = 0; r < R; ++r) o[r][dt] = mma(v, p[r][t], o[r][dt]);
           }
@@ -252,9 +252,8 @@ Plan plan_fwd(int B, int Lq, int Lk, int H, int Hkv) { return plan((long)B * Hkv
 
 template <typename T, int DK, int WQ, int R, int WK, int SUB, int JOINT>
 int launch_fwd(const MhaArgs& a, T* out, float* lse, float* part, hipStream_t st) {
-  using S = Shape<T, DK>;
-  const size_t join = WK > 1 ? (size_t)((WK - 1) * 32 * (S::W + 4) + WK * 32 * 2) * 4 : 0;
-  const size_t tiles = 2 * 32 * WK * SUB * S::ROW;
+  const size_t join = WK > 1 ? (size_t)((WK - 1) * 32 * (row_width(DK) + 4) + WK * 32 * 2) * 4 : 0;
+  const size_t tiles = 2 * Tile<T, row_width(DK), 32 * WK * SUB>::BYTES;
   size_t lds = 2 * tiles <= 64 * 1024 ? 2 * tiles : tiles;
   if (join > lds) lds = join;
   const auto kernel = mha_fwd_kernel<T, DK, WQ, R, WK, SUB, JOINT>;
@@ -266,22 +265,22 @@ int launch_fwd(const MhaArgs& a, T* out, float* lse, float* part, hipStream_t st
 
 template <typename T, int DK>
 int run_fwd(MhaArgs& a, T* out, float* lse, float* part, hipStream_t st) {
-  using S = Shape<T, DK>;
   const Plan p = plan_fwd(a.B, a.Lq, a.Lk, a.H, a.Hkv);
   a.nblk = p.nblk, a.nsplit = p.nsplit, a.per_split = p.per_split;
   if (p.nsplit == 1) part = nullptr;
+  constexpr int FSUB = sizeof(T) == 4 && DK > 64 ? 1 : 2;
   int rc;
   if (!p.wide) {
-    rc = launch_fwd<T, DK, 1, 1, S::WK, 1, 1>(a, out, lse, part, st);
+    rc = launch_fwd<T, DK, 1, 1, narrow_waves<T>(DK), 1, 1>(a, out, lse, part, st);
   } else if constexpr (sizeof(T) == 2 && DK <= 64) {
     if ((long)a.B * a.Hkv * a.nsplit * cdiv(a.rows, 256) >= 256) {
       a.nblk = cdiv(a.rows, 256);
       rc = launch_fwd<T, DK, 4, 2, 1, 2, 2>(a, out, lse, part, st);
     } else {
-      rc = launch_fwd<T, DK, 4, 1, 1, 2, 2>(a, out, lse, part, st);
+      rc = launch_fwd<T, DK, 4, 1, 1, FSUB, FSUB>(a, out, lse, part, st);
     }
   } else {
-    rc = launch_fwd<T, DK, 4, 1, 1, 2, 2>(a, out, lse, part, st);
+    rc = launch_fwd<T, DK, 4, 1, 1, FSUB, FSUB>(a, out, lse, part, st);
   }
   if (rc) return rc;
   if (part) {

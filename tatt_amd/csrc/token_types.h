@@ -22,29 +22,14 @@ __device__ __forceinline__ bf16_t from_f32<bf16_t>(float x) {
   return *reinterpret_cast<const bf16_t*>(&b);
 }
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
+// elements of 16 bytes
 template <typename T>
-struct Elem;
-
-template <>
-struct Elem<bf16_t> {
-  typedef bf16x8 Frag;                 // 8 contraction places of one lane
-  static constexpr int PER_CHUNK = 8;  // elements of 16 bytes
-  static constexpr int STEP = 16;      // contraction places of an MFMA step (both lane halves)
-};
-template <>
-struct Elem<float> {
-  typedef f32x4 Frag;
-  static constexpr int PER_CHUNK = 4;
-  static constexpr int STEP = 8;
-};
+constexpr int per_chunk() { return 16 / (int)sizeof(T); }
 
 // chunk `c` of a row of D elements, zeros behind its end
 template <typename T>
 __device__ __forceinline__ uint4 load_chunk(const T* row, int c, int D, int vec) {
-  constexpr int E = Elem<T>::PER_CHUNK;
+  constexpr int E = per_chunk<T>();
   uint4 r = make_uint4(0, 0, 0, 0);
   if (vec) {
     if (c * E < D) r = *reinterpret_cast<const uint4*>(row + c * E);
