@@ -389,12 +389,13 @@ int tatt_rotary(const void* q, const long* q_strides, void* q_out, int Hq, const
  * backward call: and out, dout, 15 values); rows of whole 16 bytes at 16-byte aligned places (pad D with zeros, which add nothing), 128 rows
  * (tokens x heads of a group) within 2^31 bytes.  key_mask (may be NULL): bytes [B][Lk], not 0 = leave the key out, mask_strides (batch, key).  causal: query i
  * sees key j iff j <= i + Lk - Lq.  out contiguous [B][Lq][H][D]; lse [B][H][Lq] = base-2 logarithm of the sum of the
- * exponentials (NULL if no backward call follows).  A row that sees no key gives zeros, lse = +inf, and no gradient.  The backward call recomputes the probabilities from lse; dq, dk, dv contiguous.
+ * exponentials, and, for bf16 tensors, out_low like out = what rounding took from out, which the backward call adds again in its row sums dO . O (both NULL
+ * if no backward call follows; out_low may be).  A row that sees no key gives zeros, lse = +inf, and no gradient.  The backward call recomputes the probabilities from lse; dq, dk, dv contiguous.
  * workspace: tatt_mha_*_workspace floats (0 = may be NULL). */
 size_t tatt_mha_fwd_workspace(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype);
-int tatt_mha_fwd(const void* q, const void* k, const void* v, const long* strides, const unsigned char* key_mask, const long* mask_strides, void* out, float* lse, int B, int Lq, int Lk, int H, int Hkv, int D, float scale, int causal, int dtype, float* workspace, hipStream_t stream);
+int tatt_mha_fwd(const void* q, const void* k, const void* v, const long* strides, const unsigned char* key_mask, const long* mask_strides, void* out, void* out_low, float* lse, int B, int Lq, int Lk, int H, int Hkv, int D, float scale, int causal, int dtype, float* workspace, hipStream_t stream);
 size_t tatt_mha_bwd_workspace(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype);
-int tatt_mha_bwd(const void* q, const void* k, const void* v, const long* strides, const unsigned char* key_mask, const long* mask_strides, const void* out, const void* dout, const float* lse, void* dq, void* dk, void* dv, int B, int Lq, int Lk, int H, int Hkv, int D, float scale, int causal, int dtype, float* workspace, hipStream_t stream);
+int tatt_mha_bwd(const void* q, const void* k, const void* v, const long* strides, const unsigned char* key_mask, const long* mask_strides, const void* out, const void* out_low, const void* dout, const float* lse, void* dq, void* dk, void* dv, int B, int Lq, int Lk, int H, int Hkv, int D, float scale, int causal, int dtype, float* workspace, hipStream_t stream);
 
 #ifdef __cplusplus
 }

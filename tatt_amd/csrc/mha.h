@@ -2,7 +2,7 @@
 // arguments, their checks and the launch plans.
 //
 //   S = log2(e) scale q k^T;  lse_i = log2 sum_j 2^S_ij;  P = 2^(S - lse);  O = P V
-//   delta_i = dO_i . O_i;  dV = P^T dO;  dS = P (dO V^T - delta);  dQ = scale dS K;  dK = scale dS^T Q
+//   delta_i = dO_i . O_i (bf16: of O as two bf16 numbers; the rounding of O alone would be most of the gradients' error where a row sees few keys);  dV = P^T dO;  dS = P (dO V^T - delta);  dQ = scale dS K;  dK = scale dS^T Q
 // lse stays in base 2 between the passes: a change of base would round it twice more, and P is off by lse times those roundings.
 // H = G * Hkv query heads: head h reads key head h / G.  The G heads of a key head are rows of the same problem (row = query * G + head), so a
 // single query of G heads fills G rows of a tile, and a key's gradient sums over its heads as it sums over queries.
@@ -174,6 +174,7 @@ struct Tile {
 
 struct MhaArgs {
   const void *q, *k, *v, *out, *dout;
+  const void* out_low;  // bf16: what rounding took from out (contiguous), for delta
   long qs[3], ks[3], vs[3], os[3], dos[3];  // element strides: batch, token, head
   const unsigned char* mask;
   long mask_sb, mask_sl;
@@ -394,6 +395,26 @@ __device__ __forceinline__ void store_row(T* dst, const f32x16 (&o)[ND], float f
 }
 
 // over a lane and the one 32 further: v_permlane32_swap_b32, a register exchange (a shuffle through LDS waits some hundred cycles)
+// what rounding to bf16 took from that row
+template <int ND>
+__device__ __forceinline__ void store_low(bf16_t* dst, const f32x16 (&o)[ND], float f, int D, int lane) {
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d = 32 * dt + 8 * q + 4 * (lane >> 5);
+      if (d >= D) continue;
+      uint32_t u[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float a = o[dt][4 * q + 2 * e] * f, b = o[dt][4 * q + 2 * e + 1] * f;
+        const uint32_t h = pack2(a, b);
+        u[e] = pack2(a - low2(h), b - high2(h));
+      }
+      *reinterpret_cast<uint2*>(dst + d) = make_uint2(u[0], u[1]);
+    }
+}
+
 __device__ __forceinline__ float half_max(float x) {
   const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));

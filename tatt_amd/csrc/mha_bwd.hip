@@ -36,7 +36,8 @@ __global__ __launch_bounds__(64 * WQ, dq_waves<T>(DK)) void mha_dq_kernel(MhaArg
     gf[r].load((const T*)a.dout + w.b * a.dos[0] + query[r] * a.dos[1] + h * a.dos[2], on, a.D, lane);
     if (a.scale < 0.f) qf[r].negate();
     const T* orow = (const T*)a.out + w.b * a.os[0] + query[r] * a.os[1] + h * a.os[2];
-    const float d = gf[r].dot(orow, on, a.D, lane);
+    float d = gf[r].dot(orow, on, a.D, lane);
+    if (sizeof(T) == 2 && a.out_low) d += gf[r].dot((const T*)a.out_low + at_row[r] * a.D, on, a.D, lane);
     const long stat = (w.b * a.H + h) * a.Lq + query[r];
     lse[r] = on ? a.lse[stat] : INFINITY;
     delta[r] = lse[r] == INFINITY ? 0.f : half_sum(d);  // a row that sees nothing: whatever dO holds there
@@ -381,13 +382,14 @@ size_t tatt_mha_bwd_workspace(int B, int Lq, int Lk, int H, int Hkv, int D, int 
 }
 
 int tatt_mha_bwd(const void* q, const void* k, const void* v, const long* strides, const unsigned char* mask, const long* mask_strides,
-                 const void* out, const void* dout, const float* lse, void* dq, void* dk, void* dv, int B, int Lq, int Lk, int H, int Hkv, int D,
+                 const void* out, const void* out_low, const void* dout, const float* lse, void* dq, void* dk, void* dv, int B, int Lq, int Lk, int H, int Hkv, int D,
                  float scale, int causal, int dtype, float* workspace, hipStream_t st) {
   MhaArgs a = {};
   TATT_CHECK_ARG(out && dout && lse && dq && dk && dv && workspace, "tatt_mha_bwd: bad arguments (workspace: tatt_mha_bwd_workspace floats)");
   if (int rc = fill(a, "tatt_mha_bwd", q, k, v, out, dout, strides, mask, mask_strides, B, Lq, Lk, H, Hkv, D, scale, causal, dtype, workspace)) return rc;
   TATT_CHECK_ARG((((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) == 0, "tatt_mha_bwd: dq, dk and dv are 16-byte aligned");
-  a.lse = lse, a.delta = workspace;
+  TATT_CHECK_ARG(!out_low || (dtype == TATT_T_BF16 && ((uintptr_t)out_low & 15) == 0), "tatt_mha_bwd: out_low is a 16-byte aligned bf16 tensor beside bf16 ones");
+  a.lse = lse, a.delta = workspace, a.out_low = out_low;
   float* part = workspace + ((size_t)B * H * Lq + 3) / 4 * 4;
   TATT_DISPATCH_TYPE(dtype, TATT_DISPATCH_WIDTH(D, return (run_bwd<T, DK>(a, (T*)dq, (T*)dk, (T*)dv, part, st)););;);
   return TATT_OK;

@@ -9,7 +9,7 @@ constexpr float LAZY = 8.f;       // the running maximum follows only rises of m
 
 // WQ waves along the rows (32 R each) x WK along the keys; tiles of 32 SUB keys for a wave, JOINT of them sharing a look at the maximum.
 template <typename T, int DK, int WQ, int R, int WK, int SUB, int JOINT>
-__global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel(MhaArgs a, T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part) {
+__global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel(MhaArgs a, T* __restrict__ out, bf16_t* __restrict__ low, float* __restrict__ lse, float* __restrict__ part) {
   constexpr int NT = 64 * WQ * WK, W = row_width(DK), ND = (DK + 31) / 32, KT = 32 * WK * SUB, TILE = Tile<T, W, KT>::BYTES;
   constexpr int NS = DK / STEP, TS = 32 / STEP, NB = 4 * TILE <= 64 * 1024 ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -208,7 +208,9 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
         ml[0] = m[r], ml[1] = l[r];
       }
     } else {
-      store_row<T, ND>(out + at * a.D, o[r], l[r] == 0.f ? 0.f : 1.f / l[r], a.D, lane);
+      const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+      store_row<T, ND>(out + at * a.D, o[r], inv, a.D, lane);
+      if (sizeof(T) == 2 && low) store_low<ND>(low + at * a.D, o[r], inv, a.D, lane);
       if (lse && half == 0) lse[(w.b * a.H + h) * a.Lq + query[r]] = l[r] == 0.f ? INFINITY : m[r] + log2f(l[r]);
     }
   }
@@ -216,7 +218,8 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
 
 // the splits of a row: a wave per row, lane = split for the weights, then lane = dimension
 template <typename T>
-__global__ __launch_bounds__(256) void mha_fwd_join(const float* __restrict__ part, int nsplit, long R, int D, int H, int Lq, T* __restrict__ out, float* __restrict__ lse) {
+__global__ __launch_bounds__(256) void mha_fwd_join(const float* __restrict__ part, int nsplit, long R, int D, int H, int Lq, T* __restrict__ out, bf16_t* __restrict__ low,
+                                                    float* __restrict__ lse) {
   const int lane = threadIdx.x & 63;
   const long r = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= R) return;
@@ -243,49 +246,55 @@ __global__ __launch_bounds__(256) void mha_fwd_join(const float* __restrict__ pa
   }
   l = wave_sum(l);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (lane < D) out[r * D + lane] = from_f32<T>(o0 * inv);
-  if (lane + 64 < D) out[r * D + lane + 64] = from_f32<T>(o1 * inv);
+  o0 *= inv, o1 *= inv;
+  const T h0 = from_f32<T>(o0), h1 = from_f32<T>(o1);
+  if (lane < D) out[r * D + lane] = h0;
+  if (lane + 64 < D) out[r * D + lane + 64] = h1;
+  if (sizeof(T) == 2 && low) {
+    if (lane < D) low[r * D + lane] = from_f32<bf16_t>(o0 - to_f32(h0));
+    if (lane + 64 < D) low[r * D + lane + 64] = from_f32<bf16_t>(o1 - to_f32(h1));
+  }
   if (lse && lane == 0) lse[(r / H / Lq * H + r % H) * Lq + r / H % Lq] = l == 0.f ? INFINITY : m + log2f(l);
 }
 
 Plan plan_fwd(int B, int Lq, int Lk, int H, int Hkv) { return plan((long)B * Hkv, Lq * (H / Hkv), Lk); }
 
 template <typename T, int DK, int WQ, int R, int WK, int SUB, int JOINT>
-int launch_fwd(const MhaArgs& a, T* out, float* lse, float* part, hipStream_t st) {
+int launch_fwd(const MhaArgs& a, T* out, bf16_t* low, float* lse, float* part, hipStream_t st) {
   const size_t join = WK > 1 ? (size_t)((WK - 1) * 32 * (row_width(DK) + 4) + WK * 32 * 2) * 4 : 0;
   const size_t tiles = 2 * Tile<T, row_width(DK), 32 * WK * SUB>::BYTES;
   size_t lds = 2 * tiles <= 64 * 1024 ? 2 * tiles : tiles;
   if (join > lds) lds = join;
   const auto kernel = mha_fwd_kernel<T, DK, WQ, R, WK, SUB, JOINT>;
   if (int rc = prepare_launch(a, kernel, 64 * WQ * WK, lds)) return rc;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)((long)a.B * a.Hkv * a.nblk * a.nsplit)), dim3(64 * WQ * WK), lds, st, a, out, lse, part);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((long)a.B * a.Hkv * a.nblk * a.nsplit)), dim3(64 * WQ * WK), lds, st, a, out, low, lse, part);
   TATT_LAUNCH_CHECK("mha_fwd");
   return TATT_OK;
 }
 
 template <typename T, int DK>
-int run_fwd(MhaArgs& a, T* out, float* lse, float* part, hipStream_t st) {
+int run_fwd(MhaArgs& a, T* out, bf16_t* low, float* lse, float* part, hipStream_t st) {
   const Plan p = plan_fwd(a.B, a.Lq, a.Lk, a.H, a.Hkv);
   a.nblk = p.nblk, a.nsplit = p.nsplit, a.per_split = p.per_split;
   if (p.nsplit == 1) part = nullptr;
   constexpr int FSUB = sizeof(T) == 4 && DK > 64 ? 1 : 2;
   int rc;
   if (!p.wide) {
-    rc = launch_fwd<T, DK, 1, 1, narrow_waves<T>(DK), 1, 1>(a, out, lse, part, st);
+    rc = launch_fwd<T, DK, 1, 1, narrow_waves<T>(DK), 1, 1>(a, out, low, lse, part, st);
   } else if constexpr (sizeof(T) == 2 && DK <= 64) {
     if ((long)a.B * a.Hkv * a.nsplit * cdiv(a.rows, 256) >= 256) {
       a.nblk = cdiv(a.rows, 256);
-      rc = launch_fwd<T, DK, 4, 2, 1, 2, 2>(a, out, lse, part, st);
+      rc = launch_fwd<T, DK, 4, 2, 1, 2, 2>(a, out, low, lse, part, st);
     } else {
-      rc = launch_fwd<T, DK, 4, 1, 1, FSUB, FSUB>(a, out, lse, part, st);
+      rc = launch_fwd<T, DK, 4, 1, 1, FSUB, FSUB>(a, out, low, lse, part, st);
     }
   } else {
-    rc = launch_fwd<T, DK, 4, 1, 1, FSUB, FSUB>(a, out, lse, part, st);
+    rc = launch_fwd<T, DK, 4, 1, 1, FSUB, FSUB>(a, out, low, lse, part, st);
   }
   if (rc) return rc;
   if (part) {
     const long R = (long)a.B * a.H * a.Lq;
-    hipLaunchKernelGGL(mha_fwd_join<T>, dim3(cdiv(R, 4)), dim3(256), 0, st, part, a.nsplit, R, a.D, a.H, a.Lq, out, lse);
+    hipLaunchKernelGGL(mha_fwd_join<T>, dim3(cdiv(R, 4)), dim3(256), 0, st, part, a.nsplit, R, a.D, a.H, a.Lq, out, low, lse);
     TATT_LAUNCH_CHECK("mha_fwd_join");
   }
   return TATT_OK;
@@ -302,12 +311,13 @@ size_t tatt_mha_fwd_workspace(int B, int Lq, int Lk, int H, int Hkv, int D, int 
 }
 
 int tatt_mha_fwd(const void* q, const void* k, const void* v, const long* strides, const unsigned char* mask, const long* mask_strides,
-                 void* out, float* lse, int B, int Lq, int Lk, int H, int Hkv, int D, float scale, int causal, int dtype, float* workspace,
+                 void* out, void* out_low, float* lse, int B, int Lq, int Lk, int H, int Hkv, int D, float scale, int causal, int dtype, float* workspace,
                  hipStream_t st) {
   MhaArgs a = {};
   if (int rc = fill(a, "tatt_mha_fwd", q, k, v, out, nullptr, strides, mask, mask_strides, B, Lq, Lk, H, Hkv, D, scale, causal, dtype, workspace)) return rc;
+  TATT_CHECK_ARG(!out_low || (dtype == TATT_T_BF16 && ((uintptr_t)out_low & 15) == 0), "tatt_mha_fwd: out_low is a 16-byte aligned bf16 tensor beside bf16 ones");
   TATT_CHECK_ARG(workspace || tatt_mha_fwd_workspace(B, Lq, Lk, H, Hkv, D, dtype) == 0, "tatt_mha_fwd: needs tatt_mha_fwd_workspace floats");
-  TATT_DISPATCH_TYPE(dtype, TATT_DISPATCH_WIDTH(D, return (run_fwd<T, DK>(a, (T*)out, lse, workspace, st)););;);
+  TATT_DISPATCH_TYPE(dtype, TATT_DISPATCH_WIDTH(D, return (run_fwd<T, DK>(a, (T*)out, (bf16_t*)out_low, lse, workspace, st)););;);
   return TATT_OK;
 }
 

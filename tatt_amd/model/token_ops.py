@@ -246,61 +246,66 @@ def _laid_out(t, dtype, group=1):
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def attention_forward(q, k, v, key_padding_mask=None, causal=False, scale=None, need_lse=True):
-    """-> (out, lse): `attention` without autograd; lse [B, H, Lq] fp32 (None unless need_lse), the base-2
-    logarithm of each row's sum of exponentials (+inf where it sees nothing), is what attention_backward recomputes from."""
+def attention_forward(q, k, v, key_padding_mask=None, causal=False, scale=None, need_saved=True):
+    """-> (out, saved): `attention` without autograd; saved = (lse, low) is what attention_backward recomputes from (None unless need_saved): lse
+    [B, H, Lq] fp32, the base-2 logarithm of each row's sum of exponentials (+inf where it sees nothing), and, for bfloat16, what rounding took from
+    out (None for float32)."""
     dtype, dims, scale = _attention_args(q, k, v, key_padding_mask, scale)
     B, Lq, Lk, H, Hk, D = dims
     if B == 0 or Lq == 0 or Lk == 0:
-        return q.new_zeros(q.shape), q.new_full((B, H, Lq), float("inf"), dtype=torch.float32) if need_lse else None
+        return q.new_zeros(q.shape), (q.new_full((B, H, Lq), float("inf"), dtype=torch.float32), None) if need_saved else None
     q, k, v = _laid_out(q, dtype, H // Hk), _laid_out(k, dtype), _laid_out(v, dtype)
     P = q.shape[3]
     dims = (B, Lq, Lk, H, Hk, P)
     out = _like(q)
-    lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device) if need_lse else None
+    lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device) if need_saved else None
+    low = _like(q) if need_saved and dtype else None
     n = lib().cdll.tatt_mha_fwd_workspace(*dims, dtype)
     ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
     mask_strides = None if key_padding_mask is None else _L2(*key_padding_mask.stride())
     _call("tatt_mha_fwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), _L9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]),
-          _ptr(key_padding_mask), mask_strides, out.data_ptr(), _ptr(lse), *dims, scale, bool(causal), dtype, _ptr(ws))
-    return out if P == D else out[..., :D].contiguous(), lse
+          _ptr(key_padding_mask), mask_strides, out.data_ptr(), _ptr(low), _ptr(lse), *dims, scale, bool(causal), dtype, _ptr(ws))
+    return out if P == D else out[..., :D].contiguous(), (lse, low) if need_saved else None
 
 
-def attention_backward(dout, q, k, v, out, lse, key_padding_mask=None, causal=False, scale=None):
-    """-> (dq, dk, dv) of attention_forward with the same arguments: the probabilities are recomputed from lse."""
+def attention_backward(dout, q, k, v, out, saved, key_padding_mask=None, causal=False, scale=None):
+    """-> (dq, dk, dv) of attention_forward with the same arguments: the probabilities are recomputed from what it saved."""
     dtype, dims, scale = _attention_args(q, k, v, key_padding_mask, scale)
     _check("attention", q, out, dout)
     B, Lq, Lk, H, Hk, D = dims
-    if out.shape != q.shape or dout.shape != q.shape or lse.shape != (B, H, Lq) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
-        raise RuntimeError("tatt_amd attention_backward: out and dout have the shape of q, lse is attention_forward's")
+    lse, low = saved
+    P = D + -D % (8 if dtype else 4)
+    if (out.shape != q.shape or dout.shape != q.shape or lse.shape != (B, H, Lq) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous()
+            or low is not None and (low.shape != (B, Lq, H, P) or low.dtype != torch.bfloat16 or not dtype or low.device != q.device or not low.is_contiguous())):
+        raise RuntimeError("tatt_amd attention_backward: out and dout have the shape of q, saved is attention_forward's")
     if B == 0 or Lq == 0 or Lk == 0:
         return q.new_zeros(q.shape), k.new_zeros(k.shape), v.new_zeros(v.shape)
     q, out, dout = (_laid_out(t, dtype, H // Hk) for t in (q, out, dout))
     k, v = _laid_out(k, dtype), _laid_out(v, dtype)
-    P = q.shape[3]
     dims = (B, Lq, Lk, H, Hk, P)
     dq, dk, dv = _like(q), _like(k), _like(v)
     ws = torch.empty(lib().cdll.tatt_mha_bwd_workspace(*dims, dtype), dtype=torch.float32, device=q.device)
     mask_strides = None if key_padding_mask is None else _L2(*key_padding_mask.stride())
     _call("tatt_mha_bwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(),
           _L15(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *dout.stride()[:3]), _ptr(key_padding_mask), mask_strides,
-          out.data_ptr(), dout.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *dims, scale, bool(causal), dtype, ws.data_ptr())
+          out.data_ptr(), _ptr(low), dout.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *dims, scale, bool(causal), dtype,
+          ws.data_ptr())
     return (dq, dk, dv) if P == D else tuple(t[..., :D].contiguous() for t in (dq, dk, dv))
 
 
 class _AttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, causal, scale):
-        out, lse = attention_forward(q, k, v, mask, causal, scale)
-        ctx.save_for_backward(q, k, v, out, lse, mask)
+        out, saved = attention_forward(q, k, v, mask, causal, scale)
+        ctx.save_for_backward(q, k, v, out, *saved, mask)
         ctx.how = (causal, scale)
         return out
 
     @staticmethod
     def backward(ctx, dout):
         _first_order("attention")
-        q, k, v, out, lse, mask = ctx.saved_tensors
-        return (*attention_backward(dout, q, k, v, out, lse, mask, *ctx.how), None, None, None)
+        q, k, v, out, lse, low, mask = ctx.saved_tensors
+        return (*attention_backward(dout, q, k, v, out, (lse, low), mask, *ctx.how), None, None, None)
 
 
 def attention(q, k, v, key_padding_mask=None, causal=False, scale=None):
@@ -310,4 +315,4 @@ def attention(q, k, v, key_padding_mask=None, causal=False, scale=None):
     that sees no key gives zeros.  -> out [B, Lq, H, D]."""
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _AttentionFn.apply(q, k, v, key_padding_mask, causal, scale)
-    return attention_forward(q, k, v, key_padding_mask, causal, scale, need_lse=False)[0]
+    return attention_forward(q, k, v, key_padding_mask, causal, scale, need_saved=False)[0]

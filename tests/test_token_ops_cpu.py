@@ -22,13 +22,13 @@ def test_cpu_tensors_are_refused():
 
 
 def fwd(**kw):
-    a = dict(q=P, k=P, v=P, strides=L9(), mask=None, mask_strides=None, out=P, lse=None, B=1, Lq=1, Lk=1, H=1, Hkv=1, D=16, scale=1.0, causal=0, dtype=0, ws=None)
+    a = dict(q=P, k=P, v=P, strides=L9(), mask=None, mask_strides=None, out=P, low=None, lse=None, B=1, Lq=1, Lk=1, H=1, Hkv=1, D=16, scale=1.0, causal=0, dtype=0, ws=None)
     a.update(kw)
     tl.lib().mha_fwd(*a.values(), None)
 
 
 def bwd(**kw):
-    a = dict(q=P, k=P, v=P, strides=L15(), mask=None, mask_strides=None, out=P, dout=P, lse=P, dq=P, dk=P, dv=P, B=1, Lq=1, Lk=1, H=1, Hkv=1, D=16,
+    a = dict(q=P, k=P, v=P, strides=L15(), mask=None, mask_strides=None, out=P, low=None, dout=P, lse=P, dq=P, dk=P, dv=P, B=1, Lq=1, Lk=1, H=1, Hkv=1, D=16,
              scale=1.0, causal=0, dtype=0, ws=P)
     a.update(kw)
     tl.lib().mha_bwd(*a.values(), None)
@@ -37,7 +37,7 @@ def bwd(**kw):
 @pytest.mark.parametrize("call", [fwd, bwd])
 @pytest.mark.parametrize("kw,text", [({"q": None}, "bad arguments"), ({"v": None}, "bad arguments"), ({"strides": None}, "bad arguments"), ({"out": None}, "mha"),
                                      ({"B": 0}, "bad arguments"), ({"Lk": 0}, "bad arguments"), ({"Lq": -3}, "bad arguments"), ({"H": 3, "Hkv": 2}, "multiple"),
-                                     ({"D": 129}, "1 to 128"), ({"D": 0}, "1 to 128"), ({"dtype": 2}, "element type"), ({"mask": P}, "strides"),
+                                     ({"low": P}, "out_low"), ({"dtype": 1, "low": P + 2}, "out_low"), ({"D": 129}, "1 to 128"), ({"D": 0}, "1 to 128"), ({"dtype": 2}, "element type"), ({"mask": P}, "strides"),
                                      ({"B": 1 << 20, "Lq": 1 << 12}, "2\\^30"), ({"B": 1 << 20, "Lk": 1 << 12}, "2\\^30")])
 def test_attention_entry_points_refuse(call, kw, text):
     with pytest.raises(RuntimeError, match=text):
