@@ -2,7 +2,9 @@
 // arguments, their checks and the launch plans.
 //
 //   S = log2(e) scale q k^T;  lse_i = log2 sum_j 2^S_ij;  P = 2^(S - lse);  O = P V
-//   delta_i = dO_i . O_i (bf16: of O as two bf16 numbers; the rounding of O alone would be most of the gradients' error where a row sees few keys);  dV = P^T dO;  dS = P (dO V^T - delta);  dQ = scale dS K;  dK = scale dS^T Q
+//   delta_i = dO_i . O_i;  dV = P^T dO;  dS = P (dO V^T - delta);  dQ = scale dS K;  dK = scale dS^T Q
+// bf16: delta is formed from O as two bf16 numbers, what is stored and what rounding took from it; without the second that rounding is most of the
+// gradients' error where a row sees few keys.
 // lse stays in base 2 between the passes: a change of base would round it twice more, and P is off by lse times those roundings.
 // H = G * Hkv query heads: head h reads key head h / G.  The G heads of a key head are rows of the same problem (row = query * G + head), so a
 // single query of G heads fills G rows of a tile, and a key's gradient sums over its heads as it sums over queries.
@@ -378,6 +380,25 @@ __device__ __forceinline__ void trim_keys(const unsigned char* mask, long stride
   hi = __builtin_amdgcn_readfirstlane(last + 1);
 }
 
+// the first key below `hi` that is not masked (`hi`: none); `red` = 4 bytes of LDS a wave
+template <int NT>
+__device__ __forceinline__ int first_key(const unsigned char* mask, long stride, int hi, int* red) {
+  int first = hi;
+  for (int j = threadIdx.x; j < hi; j += NT)
+    if (!mask[j * stride]) {
+      first = j;
+      break;
+    }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o, 64));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = first;
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < NT / 64; ++x) first = min(first, red[x]);
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(first);
+}
+
 // the D elements of one row held as accumulators of a transposed product (lane = row, registers = dimensions), times f, to dst
 template <typename T, int ND>
 __device__ __forceinline__ void store_row(T* dst, const f32x16 (&o)[ND], float f, int D, int lane) {
@@ -394,7 +415,6 @@ __device__ __forceinline__ void store_row(T* dst, const f32x16 (&o)[ND], float f
     }
 }
 
-// over a lane and the one 32 further: v_permlane32_swap_b32, a register exchange (a shuffle through LDS waits some hundred cycles)
 // what rounding to bf16 took from that row
 template <int ND>
 __device__ __forceinline__ void store_low(bf16_t* dst, const f32x16 (&o)[ND], float f, int D, int lane) {
@@ -415,6 +435,7 @@ __device__ __forceinline__ void store_low(bf16_t* dst, const f32x16 (&o)[ND], fl
     }
 }
 
+// over a lane and the one 32 further: v_permlane32_swap_b32, a register exchange (a shuffle through LDS waits some hundred cycles)
 __device__ __forceinline__ float half_max(float x) {
   const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));

@@ -163,10 +163,11 @@ __global__ __launch_bounds__(64 * WN * WR, dkv_waves<T>(DK)) void mha_dkv_kernel
   const float* lse = a.lse + (w.b * a.H + w.hk * a.G) * a.Lq;
   const float* delta = a.delta + (w.b * a.H + w.hk * a.G) * a.Lq;
 
-  // causal: this key is seen from row G (key - past) on; rows before the first query that sees anything hold what they like
+  // causal: this key is seen from row G (key - past) on; rows before the first query that sees an unmasked key hold what they like
   const int first_row = a.causal ? a.G * max(0, key - past) : 0;
   const int all_rows = a.causal ? a.G * max(0, key0 + 32 * wn + 31 - past) : 0;  // from here on every key of the wave is seen
-  const int empty_rows = a.causal ? a.G * max(0, -past) : 0;
+  const int first_seen = a.causal && a.mask ? first_key<NT>(a.mask + w.b * a.mask_sb, a.mask_sl, min(a.Lk, key0 + 32 * WN), reinterpret_cast<int*>(lds)) : 0;
+  const int empty_rows = a.causal ? a.G * max(0, first_seen - past) : 0;
   const bool whole = __all(on);
   int rbeg = w.split * a.per_split;
   const int rend = min(a.rows, rbeg + a.per_split);

@@ -4,7 +4,10 @@
 
 namespace {
 
-constexpr float NO_MAX = -1e30f;  // the running maximum before any visible score; finite, so that differences from it are not NaN
+constexpr float NO_MAX = -3.40282347e38f;  // the running maximum before any visible score: the lowest number, finite so that differences from it are not NaN
+// A maximum this far from 0 makes its row NaN: the product of score and scale is rounded in the maximum and not in the difference from it, and past
+// 2^31 that residue (2^-24 of it) leaves the range of the exponential, so that the row would come out as zeros or infinities by chance.
+constexpr float FAR = 536870912.f;  // 2^29
 constexpr float LAZY = 8.f;       // the running maximum follows only rises of more than 2^8: P stays below 2^8, and fp32 sums hold that exactly as well
 
 // WQ waves along the rows (32 R each) x WK along the keys; tiles of 32 SUB keys for a wave, JOINT of them sharing a look at the maximum.
@@ -113,7 +116,9 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
       if (__any(rise)) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const float mn = fmaxf(m[r], tmax[r]), f = __builtin_amdgcn_exp2f(m[r] - mn);
+          float mn = fmaxf(m[r], tmax[r]);
+          if (fabsf(mn) >= FAR && mn != NO_MAX) mn = NAN;
+          const float f = __builtin_amdgcn_exp2f(m[r] - mn);
           m[r] = mn;
           l[r] *= f;
 #pragma unroll

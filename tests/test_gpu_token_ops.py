@@ -190,6 +190,44 @@ def test_attention_rows_that_see_nothing_take_no_part(dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(2, 90, 90, 4, 2, 32), (2, 40, 300, 4, 4, 128), (2, 600, 20, 2, 1, 64)], ids=lambda s: "x".join(map(str, s)))
+def test_attention_rows_that_see_only_masked_keys_take_no_part(shape, dtype):
+    """Causal with padding in front: the first rows see masked keys alone, whatever their q and dout hold."""
+    B, Lq, Lk, H, Hk, D = shape
+    q, k, v = heads("tokens", *shape, dtype, 6)
+    do = rnd(B, Lq, H, D, seed=9, dtype=dtype)
+    first = Lk - Lq + 30 if Lk > 30 else 10           # the first key that is not masked; row 0 sees Lk - Lq + 1 keys
+    mask = (torch.arange(Lk) < torch.tensor([[first], [0]])).cuda()
+    blind = first - (Lk - Lq)                         # rows of the first sequence that see nothing
+    want = T.attention_forward(q, k, v, mask, True)
+    ref = T.attention_backward(do, q, k, v, *want, mask, True)
+    do[0, :blind], q[0, :blind] = float("nan"), float("inf")
+    out, saved = T.attention_forward(q, k, v, mask, True)
+    got = T.attention_backward(do, q, k, v, out, saved, mask, True)
+    assert torch.equal(out, want[0]) and not out[0, :blind].any() and torch.isinf(saved[0][0, :, :blind]).all() and torch.isfinite(saved[0][0, :, blind:]).all()
+    assert not got[0][0, :blind].any()
+    for a, b in zip(got, ref):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("Lq", [1, 70])
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("size", [5e3, 1e16])
+def test_attention_scores_far_from_zero(dtype, Lq, sign, size):
+    """Scores whose steps are too large for more than one key: up to 2^29 the choice of that key; past it NaN, never a row of zeros."""
+    k = (torch.linspace(2, 1, 40) * sign * size).to(dtype).cuda()[None, :, None, None].expand(2, 40, 2, 16)
+    q, v = torch.full((2, Lq, 2, 16), size, dtype=dtype, device="cuda"), rnd(2, 40, 2, 16, seed=1, dtype=dtype)
+    out, saved = T.attention_forward(q, k, v)
+    if size == 1e16:
+        assert torch.isnan(out).all() and torch.isnan(saved[0]).all()
+        assert all(torch.isnan(g).all() for g in T.attention_backward(torch.ones_like(q), q, k, v, out, saved))
+        return
+    pick = v[:, 0 if sign > 0 else 39][:, None].expand_as(out).double().cpu()
+    within(out, pick, pick.abs(), dtype, "the chosen value")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
 @pytest.mark.parametrize("scale", [40.0, 0.0, -0.25])
 def test_attention_large_and_odd_scales(scale, dtype):
     """Scores of some hundreds: the softmax is nearly a choice of one key; 0: the mean of the values; negative: the other way round."""
