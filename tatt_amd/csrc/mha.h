@@ -532,7 +532,7 @@ int prepare_launch(const MhaArgs& a, K kernel, int threads, size_t bytes) {
   return TATT_OK;
 }
 
-// waves along the summed axis where the other axis has one tile: two tiles of 32 of their rows within 64 KB
+// waves along the summed axis where the other axis has one tile: tiles of 32 of their rows, two buffers of them within 64 KB
 template <typename T>
 constexpr int narrow_waves(int DK) { return sizeof(T) == 2 ? (DK > 64 ? 2 : 4) : (DK > 64 ? 1 : DK > 32 ? 2 : 4); }
 

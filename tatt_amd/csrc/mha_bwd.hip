@@ -362,7 +362,16 @@ int run_bwd(MhaArgs& a, T* dq, T* dk, T* dv, float* part, hipStream_t st) {
   p = plan_dkv(a.B, a.Lq, a.Lk, a.H, a.Hkv);
   a.nblk = p.nblk, a.nsplit = p.nsplit, a.per_split = p.per_split;
   float* kv_part = a.nsplit > 1 ? part : nullptr;
-  if ((rc = p.wide ? launch_dkv<T, DK, 4, 1, (sizeof(T) == 4 ? 1 : DK > 64 ? 2 : 4)>(a, dk, dv, kv_part, st) : launch_dkv<T, DK, 1, narrow_waves<T>(DK), 1>(a, dk, dv, kv_part, st))) return rc;
+  // Few keys: waves along the rows.  fp32 heads wider than 64 have no registers for that, three of four waves that only bring tiles are better
+  // (26 keys, 16 x 1024 queries, 4 heads of 128: 218 us against 361 the pass; 8 heads of 64 with 4 waves 35 us, with 2 that leave room for a second
+  // buffer 45)
+  if constexpr (sizeof(T) == 4 && DK > 64)
+    rc = launch_dkv<T, DK, 4, 1, 1>(a, dk, dv, kv_part, st);
+  else if (p.wide)
+    rc = launch_dkv<T, DK, 4, 1, (sizeof(T) == 4 ? 1 : DK > 64 ? 2 : 4)>(a, dk, dv, kv_part, st);
+  else
+    rc = launch_dkv<T, DK, 1, (sizeof(T) == 4 ? 4 : narrow_waves<T>(DK)), 1>(a, dk, dv, kv_part, st);
+  if (rc) return rc;
   if (kv_part) {
     const long n = (long)a.B * a.Hkv * a.Lk * a.D;
     hipLaunchKernelGGL(mha_sum_kernel<T>, dim3(cdiv(2 * n, 256)), dim3(256), 0, st, part, a.nsplit, n, dk, dv);

@@ -284,8 +284,12 @@ int run_fwd(MhaArgs& a, T* out, bf16_t* low, float* lse, float* part, hipStream_
   if (p.nsplit == 1) part = nullptr;
   constexpr int FSUB = sizeof(T) == 4 && DK > 64 ? 1 : 2;
   int rc;
+  constexpr int WK = narrow_waves<T>(DK), MORE = sizeof(T) == 4 && DK > 32 ? 2 * WK : WK;
   if (!p.wide) {
-    rc = launch_fwd<T, DK, 1, 1, narrow_waves<T>(DK), 1, 1>(a, out, low, lse, part, st);
+    // fp32 tiles of wide heads leave no room for a second buffer beside more waves.  Where the keys are split over workgroups, the other workgroups
+    // fill a wave's waits; where they are not, more waves do (8 x 32 heads of 128, one query: 300 keys 48 us with 1 wave and 30 with 2, 20000 keys
+    // 385 and 440)
+    rc = p.nsplit > 1 ? launch_fwd<T, DK, 1, 1, WK, 1, 1>(a, out, low, lse, part, st) : launch_fwd<T, DK, 1, 1, MORE, 1, 1>(a, out, low, lse, part, st);
   } else if constexpr (sizeof(T) == 2 && DK <= 64) {
     if ((long)a.B * a.Hkv * a.nsplit * cdiv(a.rows, 256) >= 256) {
       a.nblk = cdiv(a.rows, 256);
