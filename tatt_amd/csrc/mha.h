@@ -500,6 +500,7 @@ inline int fill(MhaArgs& a, const char* who, const void* q, const void* k, const
   TATT_CHECK_ARG(q && k && v && out && strides && B > 0 && Lq > 0 && Lk > 0 && H > 0 && Hkv > 0, "%s: bad arguments", who);
   TATT_CHECK_ARG(!mask || mask_strides, "%s: a key mask needs its strides", who);
   TATT_CHECK_ARG(H % Hkv == 0, "%s: %d query heads are no multiple of %d key heads", who, H, Hkv);
+  TATT_CHECK_ARG(H / Hkv <= 1 << 16, "%s: %d query heads to %d key heads, more than 65536 to one", who, H, Hkv);
   TATT_CHECK_ARG(D > 0 && D <= 128, "%s: built for heads of 1 to 128, got %d", who, D);
   TATT_CHECK_ARG(dtype == TATT_T_F32 || dtype == TATT_T_BF16, "%s: unknown element type %d", who, dtype);
   TATT_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "%s: the workspace is not 16-byte aligned", who);

@@ -50,7 +50,7 @@ struct alignas(sizeof(T) * (FITS ? V : 1)) Vec {
 template <typename T, int V, bool INTERLEAVED, bool FITS>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   __shared__ float2 turns[TURNS];
-  const int token0 = blockIdx.x * a.per_block, n = min(a.per_block, a.tokens - token0);
+  const int token0 = (int)blockIdx.x * a.per_block, n = min(a.per_block, a.tokens - token0);
   const int rest = a.D - 2 * a.pairs, heads = a.H[0] + a.H[1];
   // units of a head: V pairs each (halves: V elements of either half), then V elements each of what passes through
   constexpr int PAIRS = INTERLEAVED ? V / 2 : V, REST = FITS ? V : 1;
@@ -120,7 +120,7 @@ bool fits(const RotaryArgs& a, int V, int size, int interleaved) {
 
 template <typename T, bool INTERLEAVED>
 void launch(const RotaryArgs& a, hipStream_t st) {
-  const unsigned n = (a.tokens + a.per_block - 1) / a.per_block;
+  const unsigned n = cdiv(a.tokens, a.per_block);
   constexpr int V = 16 / sizeof(T);
   if (fits(a, V, sizeof(T), INTERLEAVED))
     hipLaunchKernelGGL((rotary_kernel<T, V, INTERLEAVED, true>), dim3(n), dim3(256), 0, st, a);
@@ -159,7 +159,7 @@ int tatt_rotary(const void* q, const long* q_strides, void* q_out, int Hq, const
   // as many tokens as LDS holds turns for, but no fewer than 1024 workgroups where there are tokens for them: few tokens wait for nothing but latency
   int per = TURNS / a.pairs, most = a.tokens / 1024;
   a.per_block = per < 1 || most < 1 ? 1 : per < most ? per : most;
-  while ((a.tokens + a.per_block - 1) / a.per_block >= 1 << 24) a.per_block *= 2;  // the grid's own limit
+  while (cdiv(a.tokens, a.per_block) >= 1 << 24) a.per_block *= 2;  // the grid's own limit
   TATT_DISPATCH_TYPE(dtype, if (interleaved) launch<T, true>(a, st); else launch<T, false>(a, st););
   TATT_LAUNCH_CHECK("rotary");
   return TATT_OK;

@@ -175,6 +175,8 @@ def rotate(q, k, positions, freqs, sections, interleaved=False, inverse=False):
         raise RuntimeError(f"tatt_amd rotary: positions [L, axes] or [B, L, axes] on the tensors' device expected, got {tuple(shape)} on {positions.device}")
     if freqs.dtype != torch.float64 or freqs.shape != (width // 2,) or freqs.device != device or not freqs.is_contiguous():
         raise RuntimeError("tatt_amd rotary: freqs is a contiguous float64 vector of sum(sections) / 2 on the tensors' device (rotary_frequencies)")
+    if H == 0 and k is not None:
+        return _like(q), rotate(k, None, positions, freqs, sections, interleaved, inverse)[0]
     qo, ko = _like(q), None if k is None else _like(k)
     if qo.numel():
         q, k = _rows(q), None if k is None or not ko.numel() else _rows(k)
@@ -312,7 +314,11 @@ def attention(q, k, v, key_padding_mask=None, causal=False, scale=None):
     """softmax(scale q k^T) v per head, the scores never in memory.  q [B, Lq, H, D], k and v [B, Lk, Hk, D] (float32 or bfloat16, any
     strides, D <= 128), H a multiple of Hk: query head h reads key head h // (H // Hk).  key_padding_mask [B, Lk] bool, True = leave the key out (as
     nn.MultiheadAttention's): nothing of such a key reaches a result.  causal: query i sees keys j <= i + Lk - Lq.  scale: D ** -0.5 if None.  A row
-    that sees no key gives zeros.  -> out [B, Lq, H, D]."""
+    that sees no key gives zeros and takes no part in any gradient.  -> out [B, Lq, H, D].
+
+    What is not masked is expected to be finite: an infinity or NaN spreads to what a matrix product with it would reach, the rows from which only
+    causality hides it included (0 times it).  float32 keeps its accuracy for magnitudes of 2^-100 to 2^127, scores (scaled) for magnitudes below
+    2^28, past which a row may be NaN; the gradients' probabilities are off by 2^-24 of the score, relative to themselves."""
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _AttentionFn.apply(q, k, v, key_padding_mask, causal, scale)
     return attention_forward(q, k, v, key_padding_mask, causal, scale, need_saved=False)[0]

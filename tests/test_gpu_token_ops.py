@@ -445,6 +445,16 @@ def test_rotary(D, sections, interleaved, dtype):
         assert torch.equal(qo[..., rest:], q[..., rest:]) and torch.equal(gk[..., rest:], dk[..., rest:])
 
 
+@pytest.mark.parametrize("H,Hk", [(0, 2), (2, 0), (0, 0)])
+def test_rotary_of_no_heads(H, Hk):
+    q, k = rnd(2, 5, H, 8), rnd(2, 5, Hk, 8, seed=1)
+    freqs, positions = T.rotary_frequencies((8,)), torch.arange(5, device="cuda")[:, None]
+    qo, ko = T.rotary(q, k, positions, freqs, (8,))
+    for got, x in ((qo, q), (ko, k)):
+        assert got.shape == x.shape and got.dtype == x.dtype
+        within_rotary(got, rotary_64(x, positions, (8,), False), F32, "no heads")
+
+
 @pytest.mark.parametrize("B,L,H", [(1, 1, 1), (64, 1, 32), (1, 1500, 5), (2, 1024, 4)])
 def test_rotary_sizes_one_tensor_and_one_gradient(B, L, H):
     sections, D = (16, 24, 24), 64

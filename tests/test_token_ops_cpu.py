@@ -36,7 +36,7 @@ def bwd(**kw):
 
 @pytest.mark.parametrize("call", [fwd, bwd])
 @pytest.mark.parametrize("kw,text", [({"q": None}, "bad arguments"), ({"v": None}, "bad arguments"), ({"strides": None}, "bad arguments"), ({"out": None}, "mha"),
-                                     ({"B": 0}, "bad arguments"), ({"Lk": 0}, "bad arguments"), ({"Lq": -3}, "bad arguments"), ({"H": 3, "Hkv": 2}, "multiple"),
+                                     ({"B": 0}, "bad arguments"), ({"Lk": 0}, "bad arguments"), ({"Lq": -3}, "bad arguments"), ({"H": 3, "Hkv": 2}, "multiple"), ({"H": 1 << 17}, "65536"),
                                      ({"low": P}, "out_low"), ({"dtype": 1, "low": P + 2}, "out_low"), ({"D": 129}, "1 to 128"), ({"D": 0}, "1 to 128"), ({"dtype": 2}, "element type"), ({"mask": P}, "strides"),
                                      ({"B": 1 << 20, "Lq": 1 << 12}, "2\\^30"), ({"B": 1 << 20, "Lk": 1 << 12}, "2\\^30")])
 def test_attention_entry_points_refuse(call, kw, text):
