@@ -45,9 +45,9 @@ __global__ __launch_bounds__(64 * WQ, dq_waves<T>(DK)) void mha_dq_kernel(MhaArg
     clear(o[r]);
   }
 
-  int kbeg = w.split * a.per_split;
-  int kend = min(a.Lk, kbeg + a.per_split);
+  int kbeg = 0, kend = a.Lk;
   if (a.causal) kend = min(kend, min(a.rows - 1, row0 + 32 * WQ * R - 1) / a.G + past + 1);
+  take_split(a, w.split, KT, kbeg, kend);
   if (mb && kend - kbeg > 2 * KT) trim_keys<NT>(mb, a.mask_sl, kbeg, kend, reinterpret_cast<int*>(lds));
   Stage<T, W, KT, NT, true> ks, vs;
   KeyBits<KT> next, now;
@@ -169,9 +169,8 @@ __global__ __launch_bounds__(64 * WN * WR, dkv_waves<T>(DK)) void mha_dkv_kernel
   const int first_seen = a.causal && a.mask ? first_key<NT>(a.mask + w.b * a.mask_sb, a.mask_sl, min(a.Lk, key0 + 32 * WN), reinterpret_cast<int*>(lds)) : 0;
   const int empty_rows = a.causal ? a.G * max(0, first_seen - past) : 0;
   const bool whole = __all(on);
-  int rbeg = w.split * a.per_split;
-  const int rend = min(a.rows, rbeg + a.per_split);
-  if (a.causal) rbeg = max(rbeg, a.G * max(0, key0 - past) / RT * RT);
+  int rbeg = a.causal ? a.G * max(0, key0 - past) / RT * RT : 0, rend = a.rows;
+  take_split(a, w.split, RT, rbeg, rend);
   f32x16 ok[ND], ov[ND];
   clear(ok);
   clear(ov);

@@ -18,7 +18,7 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wq = wave % WQ, wk = wave / WQ, half = lane >> 5;
   const Where w = where(a);
-  const int blk = a.causal ? a.nblk - 1 - w.blk : w.blk;  // causal: the longest blocks first
+  const int blk = a.causal ? a.nblk - 1 - w.blk : w.blk;  // causal: the last rows see most keys
   const int row0 = blk * 32 * WQ * R, wrow0 = row0 + 32 * wq * R, row = wrow0 + (lane & 31);  // and row + 32 r
   const T* kb = (const T*)a.k + w.b * a.ks[0] + w.hk * a.ks[2];
   const T* vb = (const T*)a.v + w.b * a.vs[0] + w.hk * a.vs[2];
@@ -40,9 +40,9 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
     l[r] = 0.f;
   }
 
-  int kbeg = w.split * a.per_split;
-  int kend = min(a.Lk, kbeg + a.per_split);
+  int kbeg = 0, kend = a.Lk;
   if (a.causal) kend = min(kend, min(a.rows - 1, row0 + 32 * WQ * R - 1) / a.G + past + 1);
+  take_split(a, w.split, KT, kbeg, kend);
   if (mb && kend - kbeg > 2 * KT) trim_keys<NT>(mb, a.mask_sl, kbeg, kend, reinterpret_cast<int*>(lds));
 
   Stage<T, W, KT, NT, true> ks, vs;
@@ -221,11 +221,12 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
   }
 }
 
-// the splits of a row: a wave per row, lane = split for the weights, then lane = dimension
-template <typename T>
+// The splits of a row, a wave per row.  Lane = split for the weights; then D / 4 lanes (LPR, rounded up to a power of two) hold four dimensions
+// each, and as many groups of them as the wave has take the splits in turn.  Bound by memory.
+template <typename T, int LPR>
 __global__ __launch_bounds__(256) void mha_fwd_join(const float* __restrict__ part, int nsplit, long R, int D, int H, int Lq, T* __restrict__ out, bf16_t* __restrict__ low,
                                                     float* __restrict__ lse) {
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, group = lane / LPR, d = 4 * (lane % LPR);
   const long r = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= R) return;
   const float* ml = part + nsplit * R * D;
@@ -233,33 +234,43 @@ __global__ __launch_bounds__(256) void mha_fwd_join(const float* __restrict__ pa
   for (int s = lane; s < nsplit; s += 64) m = fmaxf(m, ml[(s * R + r) * 2]);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  float l = 0.f, o0 = 0.f, o1 = 0.f;
+  float l = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s0 = 0; s0 < nsplit; s0 += 64) {
     float f = 0.f;
     if (s0 + lane < nsplit) {
-      const float2 v = *reinterpret_cast<const float2*>(ml + ((s0 + lane) * R + r) * 2);
-      f = __builtin_amdgcn_exp2f(v.x - m);
-      l += f * v.y;
+      const float2 u = *reinterpret_cast<const float2*>(ml + ((s0 + lane) * R + r) * 2);
+      f = __builtin_amdgcn_exp2f(u.x - m);
+      l += f * u.y;
     }
     const int n = min(64, nsplit - s0);
-    for (int s = 0; s < n; ++s) {
-      const float w = __shfl(f, s, 64);
-      const float* p = part + ((s0 + s) * R + r) * D;
-      if (lane < D) o0 += w * p[lane];
-      if (lane + 64 < D) o1 += w * p[lane + 64];
+    constexpr int GROUPS = 64 / LPR, AHEAD = 4;
+    for (int s = group; s - group < n; s += GROUPS * AHEAD) {
+      float4 p[AHEAD];
+#pragma unroll
+      for (int e = 0; e < AHEAD; ++e)
+        p[e] = s + e * GROUPS < n && d < D ? *reinterpret_cast<const float4*>(part + ((s0 + s + e * GROUPS) * R + r) * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int e = 0; e < AHEAD; ++e) {
+        const float w = __shfl(f, (s + e * GROUPS) & 63, 64);
+        v.x += w * p[e].x, v.y += w * p[e].y, v.z += w * p[e].z, v.w += w * p[e].w;
+      }
     }
   }
   l = wave_sum(l);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  o0 *= inv, o1 *= inv;
-  const T h0 = from_f32<T>(o0), h1 = from_f32<T>(o1);
-  if (lane < D) out[r * D + lane] = h0;
-  if (lane + 64 < D) out[r * D + lane + 64] = h1;
-  if (sizeof(T) == 2 && low) {
-    if (lane < D) low[r * D + lane] = from_f32<bf16_t>(o0 - to_f32(h0));
-    if (lane + 64 < D) low[r * D + lane + 64] = from_f32<bf16_t>(o1 - to_f32(h1));
-  }
+#pragma unroll
+  for (int o = LPR; o < 64; o *= 2) v.x += __shfl_xor(v.x, o, 64), v.y += __shfl_xor(v.y, o, 64), v.z += __shfl_xor(v.z, o, 64), v.w += __shfl_xor(v.w, o, 64);
   if (lse && lane == 0) lse[(r / H / Lq * H + r % H) * Lq + r / H % Lq] = l == 0.f ? INFINITY : m + log2f(l);
+  if (group || d >= D) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
+  if constexpr (sizeof(T) == 2) {
+    const uint2 h = make_uint2(pack2(v.x, v.y), pack2(v.z, v.w));
+    *reinterpret_cast<uint2*>(out + r * D + d) = h;
+    if (low) *reinterpret_cast<uint2*>(low + r * D + d) = make_uint2(pack2(v.x - low2(h.x), v.y - high2(h.x)), pack2(v.z - low2(h.y), v.w - high2(h.y)));
+  } else {
+    *reinterpret_cast<float4*>(out + r * D + d) = v;
+  }
 }
 
 Plan plan_fwd(int B, int Lq, int Lk, int H, int Hkv) { return plan((long)B * Hkv, Lq * (H / Hkv), Lk); }
@@ -303,7 +314,7 @@ int run_fwd(MhaArgs& a, T* out, bf16_t* low, float* lse, float* part, hipStream_
   if (rc) return rc;
   if (part) {
     const long R = (long)a.B * a.H * a.Lq;
-    hipLaunchKernelGGL(mha_fwd_join<T>, dim3(cdiv(R, 4)), dim3(256), 0, st, part, a.nsplit, R, a.D, a.H, a.Lq, out, low, lse);
+    hipLaunchKernelGGL((mha_fwd_join<T, (DK <= 16 ? 4 : DK <= 32 ? 8 : DK <= 64 ? 16 : 32)>), dim3(cdiv(R, 4)), dim3(256), 0, st, part, a.nsplit, R, a.D, a.H, a.Lq, out, low, lse);
     TATT_LAUNCH_CHECK("mha_fwd_join");
   }
   return TATT_OK;
