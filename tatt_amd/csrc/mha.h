@@ -493,14 +493,14 @@ constexpr int FILL = 512;  // workgroups that fill the 256 CUs twice
 struct Plan {
   int wide, nblk, nsplit, per_split;  // wide: waves side by side along the output axis; else along the summed one
 };
-// blocks of 128 along the output axis (32 if it has no more than 32), and the summed axis split while the chip is not full, no finer than 512
-inline Plan plan(long problems, int outer, int inner) {
+// blocks of 128 along the output axis (32 if it has no more than 32), and the summed axis split while the chip is not full, into no less than `finest`
+inline Plan plan(long problems, int outer, int inner, int finest) {
   Plan p;
   p.wide = outer > 32;
   p.nblk = cdiv(outer, p.wide ? 128 : 32);
   const long blocks = problems * p.nblk;
   long n = blocks >= FILL ? 1 : (2 * FILL + blocks - 1) / blocks;
-  if (n > inner / 512) n = inner / 512;
+  if (n > inner / finest) n = inner / finest;
   if (n < 1) n = 1;
   p.per_split = cdiv(cdiv(inner, n), 128) * 128;
   p.nsplit = cdiv(inner, p.per_split);

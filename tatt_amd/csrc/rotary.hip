@@ -5,6 +5,7 @@
 // its sine and cosine and the products are fp32.
 // Bound by memory: x is read and y written once.  The fp64 angle and the sine cost some 80 instructions, so a workgroup computes the turns of its
 // few tokens once into LDS and applies them to every head of q and k.
+// Measured: 36864 tokens, 20 heads of 128, bf16: 82 us a direction (377 MB, 4.6 TB/s); 65536 tokens, 8 heads of 16, fp32: 15-18 us (67 MB).
 #include "token_types.h"
 
 namespace {
