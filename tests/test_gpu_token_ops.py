@@ -136,6 +136,17 @@ def test_attention_masks(shape, causal, kind, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("kind", ["none", "lengths", "front"])
+@pytest.mark.parametrize("shape", [(1, 1100, 1100, 2, 2, 64), (2, 700, 1300, 4, 1, 128), (3, 1300, 600, 3, 1, 16), (1, 40, 2500, 2, 2, 96)], ids=lambda s: "x".join(map(str, s)))
+def test_attention_causal_in_splits(shape, kind, dtype):
+    """Long axes and few heads: every kernel splits the axis that it sums over, whose causal end differs from block to block."""
+    B, Lq, Lk, H, Hk, D = shape
+    q, k, v = heads("tokens", *shape, dtype, 3)
+    mask = (torch.arange(Lk) < torch.arange(B)[:, None] * (Lk // 3) + 5).cuda() if kind == "front" else key_mask(kind, B, Lk)
+    check_attention(q, k, v, rnd(B, Lq, H, D, seed=9, dtype=dtype), mask, True, D ** -0.5, kind)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
 @pytest.mark.parametrize("layout", ["packed", "heads", "odd", "apart"])
 def test_attention_layouts(layout, dtype):
     q, k, v = heads(layout, 2, 90, 90, 4, 2, 64, dtype, 3)
