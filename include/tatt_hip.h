@@ -365,7 +365,8 @@ int tatt_clip_adam(float* p, const float* g, float* m, float* v, long n, float l
 /* ---- token operators: one transformer layer over image or text tokens of any size -------------------------------------------
  * The interpreter's own layers (tatt_ln_*, tatt_attn_*, tatt_dec_*) are built for 64 channels, 4 heads x 16 and 26 keys; these take any
  * width, lengths and head counts, fp32 or bf16 tensors (`dtype` = TATT_T_F32 / TATT_T_BF16; parameters, statistics and sums fp32).
- * void* tensors are of that type; strides count elements; `strides` arguments are HOST arrays, read during the call.  No atomics: results are bit-reproducible.
+ * void* tensors are of that type; strides count elements; `strides` arguments are HOST arrays, read during the call.  Outputs and
+ * workspaces overlap nothing else; two calls in flight need a workspace each.  No atomics: results are bit-reproducible.
  *
  * LayerNorm over C columns (nn.LayerNorm at model/transformer_v2.py:478-482, :827-831, of any width), optionally with the residual sum in front:
  *   s = x + res (stored to sum, contiguous, rounded to the type; res = NULL: s = x), y = (s - mu) rstd gamma + beta (NULL: 1 / 0),
@@ -390,8 +391,9 @@ int tatt_rotary(const void* q, const long* q_strides, void* q_out, int Hq, const
  * (tokens x heads of a group) within 2^31 bytes.  key_mask (may be NULL): bytes [B][Lk], not 0 = leave the key out, mask_strides (batch, key).  causal: query i
  * sees key j iff j <= i + Lk - Lq.  out contiguous [B][Lq][H][D]; lse [B][H][Lq] = base-2 logarithm of the sum of the
  * exponentials, and, for bf16 tensors, out_low like out = what rounding took from out, which the backward call adds again in its row sums dO . O (both NULL
- * if no backward call follows; out_low may be).  A row that sees no key gives zeros, lse = +inf, and no gradient.  The backward call recomputes the probabilities from lse; dq, dk, dv contiguous.
- * workspace: tatt_mha_*_workspace floats (0 = may be NULL). */
+ * if no backward call follows; out_low may be).  A row that sees no key gives zeros, lse = +inf, and no gradient;
+ * scores past 2^29 give NaN.  The backward call recomputes the probabilities from lse; dq, dk, dv contiguous.
+ * workspace: tatt_mha_*_workspace floats, 16-byte aligned (0 = may be NULL). */
 size_t tatt_mha_fwd_workspace(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype);
 int tatt_mha_fwd(const void* q, const void* k, const void* v, const long* strides, const unsigned char* key_mask, const long* mask_strides, void* out, void* out_low, float* lse, int B, int Lq, int Lk, int H, int Hkv, int D, float scale, int causal, int dtype, float* workspace, hipStream_t stream);
 size_t tatt_mha_bwd_workspace(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype);
