@@ -488,24 +488,43 @@ __device__ __forceinline__ unsigned bits_to(int n) { return n < 0 ? 0u : n >= 31
 
 // ---- launch plans ---------------------------------------------------------------------------------------------------------------------
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int FILL = 512;  // workgroups that fill the 256 CUs twice
 
 struct Plan {
   int wide, nblk, nsplit, per_split;  // wide: waves side by side along the output axis; else along the summed one
 };
-// blocks of 128 along the output axis (32 if it has no more than 32), and the summed axis split while the chip is not full, into no less than `finest`
-inline Plan plan(long problems, int outer, int inner, int finest) {
+// Blocks of 128 along the output axis, 32 if it has no more than 32, and the summed axis in splits of no less than `finest`.
+// Few rows: as many as fill the chip twice (sequences differ in length).  Else as few as make the pass shortest, with `slots` workgroups at a time, in units
+// of a whole block: the workgroups that a CU gets one after another (of two at a time, the last alone takes 0.6), or, where causal, the longest of them
+// and their even share; and the partial sums, written and read, `traffic` / inner of the products' time a split.  (bf16, heads of 128, dK and dV: 8 x 1024
+// x 4 in 56 us unsplit and 80 + 16 in four splits, 2 x 2777 x 16 / 4 in 396 + 20 in four and 436 + 31 in six.)
+inline Plan plan(long problems, int outer, int inner, int finest, int causal, int slots, float traffic) {
   Plan p;
   p.wide = outer > 32;
   p.nblk = cdiv(outer, p.wide ? 128 : 32);
   const long blocks = problems * p.nblk;
-  long n = blocks >= FILL ? 1 : (2 * FILL + blocks - 1) / blocks;
-  if (n > inner / finest) n = inner / finest;
-  if (n < 1) n = 1;
+  long n = blocks >= slots ? 1 : (2 * slots + blocks - 1) / blocks, most = inner / finest < 1 ? 1 : inner / finest;
+  if (p.wide) {
+    const float load = (float)blocks / slots;
+    float best = 0.f;
+    long pick = 1;
+    for (long i = 1; i <= most && (i <= n || i <= 8); ++i) {
+      const float share = 0.55f * load, part = 1.f / i;
+      const int each = cdiv(blocks * i, 256);
+      const float alone = slots == 256 ? each : each == 1 ? 0.6f : 0.5f * each;
+      const float t = (causal ? (part > share ? part : share) : alone * part) + (i > 1 ? i * traffic / inner * load : 0.f);
+      if (i == 1 || t < best) best = t, pick = i;
+    }
+    n = pick;
+  }
+  if (n > most) n = most;
   p.per_split = cdiv(cdiv(inner, n), 128) * 128;
   p.nsplit = cdiv(inner, p.per_split);
   return p;
 }
+
+// workgroups of four waves that the chip holds at once, and plan()'s `traffic`: fp32 products take some five times as long
+inline int slots_of(int waves) { return waves == 1 ? 256 : 512; }
+inline float traffic_of(int dtype) { return dtype == TATT_T_BF16 ? 400.f : 80.f; }
 
 inline bool sane(int B, int Lq, int Lk, int H, int Hkv, int D) { return B > 0 && Lq > 0 && Lk > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && D > 0; }
 

@@ -319,8 +319,12 @@ __global__ __launch_bounds__(256) void mha_sum_kernel(const float* __restrict__ 
 }
 
 // Splits of no less than 256 (2 x 1024 x 1024, 4 heads of 64: fp32 70 us against 104 with 512, bf16 39 against 44; with 128 94 and 51)
-Plan plan_dq(int B, int Lq, int Lk, int H, int Hkv) { return plan((long)B * Hkv, Lq * (H / Hkv), Lk, 256); }
-Plan plan_dkv(int B, int Lq, int Lk, int H, int Hkv) { return plan((long)B * Hkv, Lk, Lq * (H / Hkv), 256); }
+Plan plan_dq(int B, int Lq, int Lk, int H, int Hkv, int D, int causal, int dtype) {
+  return plan((long)B * Hkv, Lq * (H / Hkv), Lk, 256, causal, slots_of(dtype == TATT_T_BF16 ? dq_waves<bf16_t>(D) : dq_waves<float>(D > 32 ? 64 : D)), traffic_of(dtype));
+}
+Plan plan_dkv(int B, int Lq, int Lk, int H, int Hkv, int D, int causal, int dtype) {
+  return plan((long)B * Hkv, Lk, Lq * (H / Hkv), 256, causal, slots_of(dtype == TATT_T_BF16 ? dkv_waves<bf16_t>(D) : dkv_waves<float>(D > 64 ? D : D > 32 ? 64 : D)), traffic_of(dtype));
+}
 
 template <typename T, int DK, int R, int SUB>
 int launch_dq(const MhaArgs& a, T* dq, float* part, hipStream_t st) {
@@ -345,7 +349,8 @@ int launch_dkv(const MhaArgs& a, T* dk, T* dv, float* part, hipStream_t st) {
 
 template <typename T, int DK>
 int run_bwd(MhaArgs& a, T* dq, T* dk, T* dv, float* part, hipStream_t st) {
-  Plan p = plan_dq(a.B, a.Lq, a.Lk, a.H, a.Hkv);
+  constexpr int dtype = sizeof(T) == 2 ? TATT_T_BF16 : TATT_T_F32;
+  Plan p = plan_dq(a.B, a.Lq, a.Lk, a.H, a.Hkv, a.D, a.causal, dtype);
   a.nsplit = p.nsplit, a.per_split = p.per_split;
   float* q_part = a.nsplit > 1 ? part : nullptr;
   int rc = -1;
@@ -365,7 +370,7 @@ int run_bwd(MhaArgs& a, T* dq, T* dk, T* dv, float* part, hipStream_t st) {
     hipLaunchKernelGGL(mha_sum_kernel<T>, dim3(cdiv(n, 256)), dim3(256), 0, st, part, a.nsplit, n, dq, (T*)nullptr);
     TATT_LAUNCH_CHECK("mha_sum");
   }
-  p = plan_dkv(a.B, a.Lq, a.Lk, a.H, a.Hkv);
+  p = plan_dkv(a.B, a.Lq, a.Lk, a.H, a.Hkv, a.D, a.causal, dtype);
   a.nblk = p.nblk, a.nsplit = p.nsplit, a.per_split = p.per_split;
   float* kv_part = a.nsplit > 1 ? part : nullptr;
   // Few keys: waves along the rows.  fp32 heads wider than 64 have no registers for that, three of four waves that only bring tiles are better
@@ -392,9 +397,14 @@ extern "C" {
 
 size_t tatt_mha_bwd_workspace(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype) {
   if (!sane(B, Lq, Lk, H, Hkv, D)) return 0;
-  const Plan p = plan_dq(B, Lq, Lk, H, Hkv), q = plan_dkv(B, Lq, Lk, H, Hkv);
-  const size_t a = p.nsplit == 1 ? 0 : (size_t)p.nsplit * B * H * Lq * D, b = q.nsplit == 1 ? 0 : (size_t)q.nsplit * 2 * B * Hkv * Lk * D;
-  return ((size_t)B * H * Lq + 3) / 4 * 4 + (a > b ? a : b);  // delta, then the partial sums of one kernel at a time
+  size_t most = 0;  // of either kernel, causal or not
+  for (int causal = 0; causal < 2; ++causal) {
+    const size_t p = plan_dq(B, Lq, Lk, H, Hkv, D, causal, dtype).nsplit, q = plan_dkv(B, Lq, Lk, H, Hkv, D, causal, dtype).nsplit;
+    const size_t a = p == 1 ? 0 : p * B * H * Lq * D, b = q == 1 ? 0 : q * 2 * B * Hkv * Lk * D;
+    most = a > most ? a : most;
+    most = b > most ? b : most;
+  }
+  return ((size_t)B * H * Lq + 3) / 4 * 4 + most;  // delta, then the partial sums of one kernel at a time
 }
 
 int tatt_mha_bwd(const void* q, const void* k, const void* v, const long* strides, const unsigned char* mask, const long* mask_strides,

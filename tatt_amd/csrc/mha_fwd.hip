@@ -286,7 +286,10 @@ __global__ __launch_bounds__(256) void mha_fwd_join(const float* __restrict__ pa
 // A split costs its partial sums, a second launch and the workspace: with bf16 tiles, done quickly, 512 keys are worth that (8 x 8 heads of 64, one query,
 // 1000 keys: 12 us unsplit and 16 in splits of 256; 20000 keys, 32 / 8 heads of 128: 149 in splits and 447 without), with fp32 ones 128 (17 us in splits
 // of 128 and 28 of 512; one query, 4000 keys, 8 key heads of 128: 43 and 92; with two waves, below, 29).
-Plan plan_fwd(int B, int Lq, int Lk, int H, int Hkv, int dtype) { return plan((long)B * Hkv, Lq * (H / Hkv), Lk, dtype == TATT_T_BF16 ? 512 : 128); }
+Plan plan_fwd(int B, int Lq, int Lk, int H, int Hkv, int D, int causal, int dtype) {
+  const bool bf16 = dtype == TATT_T_BF16;
+  return plan((long)B * Hkv, Lq * (H / Hkv), Lk, bf16 ? 512 : 128, causal, slots_of(bf16 ? fwd_waves<bf16_t>(D) : fwd_waves<float>(D)), traffic_of(dtype));
+}
 
 template <typename T, int DK, int WQ, int R, int WK, int SUB, int JOINT>
 int launch_fwd(const MhaArgs& a, T* out, bf16_t* low, float* lse, float* part, hipStream_t st) {
@@ -303,7 +306,7 @@ int launch_fwd(const MhaArgs& a, T* out, bf16_t* low, float* lse, float* part, h
 
 template <typename T, int DK>
 int run_fwd(MhaArgs& a, T* out, bf16_t* low, float* lse, float* part, hipStream_t st) {
-  const Plan p = plan_fwd(a.B, a.Lq, a.Lk, a.H, a.Hkv, sizeof(T) == 2 ? TATT_T_BF16 : TATT_T_F32);
+  const Plan p = plan_fwd(a.B, a.Lq, a.Lk, a.H, a.Hkv, a.D, a.causal, sizeof(T) == 2 ? TATT_T_BF16 : TATT_T_F32);
   a.nblk = p.nblk, a.nsplit = p.nsplit, a.per_split = p.per_split;
   if (p.nsplit == 1) part = nullptr;
   constexpr int FSUB = sizeof(T) == 4 && DK > 64 ? 1 : 2;
@@ -312,7 +315,7 @@ int run_fwd(MhaArgs& a, T* out, bf16_t* low, float* lse, float* part, hipStream_
   if (!p.wide) {
     // fp32 tiles of wide heads leave no room for a second buffer beside more waves.  Where workgroups fill the chip, the others fill a wave's waits;
     // where they do not, more waves do (8 x 32 heads of 128, one query: 300 keys 43 us with 1 wave and 30 with 2, 20000 keys 385 and 440)
-    const bool filled = (long)a.B * a.Hkv * p.nblk * p.nsplit >= FILL;
+    const bool filled = (long)a.B * a.Hkv * p.nblk * p.nsplit >= 512;
     rc = filled ? launch_fwd<T, DK, 1, 1, WK, 1, 1>(a, out, low, lse, part, st) : launch_fwd<T, DK, 1, 1, MORE, 1, 1>(a, out, low, lse, part, st);
   } else if constexpr (sizeof(T) == 2 && DK <= 64) {  // 64 rows a wave where that leaves a workgroup to every CU (190 us against 254, above)
     if ((long)a.B * a.Hkv * a.nsplit * cdiv(a.rows, 256) >= 256) {
@@ -339,8 +342,8 @@ extern "C" {
 
 size_t tatt_mha_fwd_workspace(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype) {
   if (!sane(B, Lq, Lk, H, Hkv, D)) return 0;
-  const Plan p = plan_fwd(B, Lq, Lk, H, Hkv, dtype);
-  return p.nsplit == 1 ? 0 : (size_t)p.nsplit * B * H * Lq * (D + 2);
+  const int a = plan_fwd(B, Lq, Lk, H, Hkv, D, 0, dtype).nsplit, b = plan_fwd(B, Lq, Lk, H, Hkv, D, 1, dtype).nsplit, n = a > b ? a : b;
+  return n == 1 ? 0 : (size_t)n * B * H * Lq * (D + 2);
 }
 
 int tatt_mha_fwd(const void* q, const void* k, const void* v, const long* strides, const unsigned char* mask, const long* mask_strides,
