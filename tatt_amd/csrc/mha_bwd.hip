@@ -4,8 +4,8 @@
 //
 // Bound like the forward pass, with three products and four to an exponential.  Measured (executed products): 4 x 4096 tokens, 8 heads of 64,
 // bf16: dQ 233 us, 885 TFLOP/s (64 rows a wave; with 32: 248), dK and dV 304 us, 904 TFLOP/s (tiles of 128 rows; of 64: 351); 16 x 1024, 4 heads of 64,
-// fp32: 177 us (146) and 225 us (153); heads of 128 in bf16, 2 x 2777 tokens of 16 heads: 232 us (815) and 435 us (580: a wave has its SIMD for itself,
-// nothing fills its waits), for one causal clip of them 126 and 161 + 28 for the sum over six splits.
+// fp32: 177 us (146) and 225 us (153); heads of 128 in bf16, 2 x 2777 tokens of 16 heads: 232 us (815) and 393 + 23 for the sum over four splits
+// (640: a wave has its SIMD for itself, nothing fills its waits), for one causal clip of them 126 and 168 + 17.
 #include "mha.h"
 
 namespace {
@@ -308,7 +308,7 @@ __global__ __launch_bounds__(64 * WN * WR, dkv_waves<T>(DK)) void mha_dkv_kernel
   }
 }
 
-// y[i] = sum over splits of part[split][i] in split order; two tensors of n values each where y2.  Bound by memory (136 MB: 28 us)
+// y[i] = sum over splits of part[split][i] in split order; two tensors of n values each where y2.  Bound by memory (six splits of 23 MB: 28 us)
 template <typename T>
 __global__ __launch_bounds__(256) void mha_sum_kernel(const float* __restrict__ part, int nsplit, long n, T* __restrict__ y, T* __restrict__ y2) {
   const long i = (long)blockIdx.x * 256 + threadIdx.x, all = y2 ? 2 * n : n;
