@@ -493,17 +493,18 @@ struct Plan {
   int wide, nblk, nsplit, per_split;  // wide: waves side by side along the output axis; else along the summed one
 };
 // Blocks of 128 along the output axis, 32 if it has no more than 32, and the summed axis in splits of no less than `finest`.
-// Few rows: as many as fill the chip twice (sequences differ in length).  Else as few as make the pass shortest, with `slots` workgroups at a time, in units
-// of a whole block: the workgroups that a CU gets one after another (of two at a time, the last alone takes 0.6), or, where causal, the longest of them
-// and their even share; and the partial sums, written and read, `traffic` / inner of the products' time a split.  (bf16, heads of 128, dK and dV: 8 x 1024
-// x 4 in 56 us unsplit and 80 + 16 in four splits, 2 x 2777 x 16 / 4 in 396 + 20 in four and 436 + 31 in six.)
-inline Plan plan(long problems, int outer, int inner, int finest, int causal, int slots, float traffic) {
+// One tile of rows: as many splits as fill the chip twice (sequences differ in length).  `whole`, workgroups that work on 128: as few as make the pass
+// shortest, with `slots` workgroups at a time, in units of a whole block: the workgroups that a CU gets one after another (of two at a time, the last alone
+// takes 0.6), or, where causal, the longest of them and their even share; and the partial sums, written and read, `traffic` / inner of the products' time a
+// split.  (bf16, heads of 128, dK and dV: 8 x 1024 x 4 in 56 us unsplit and 80 + 16 in four splits, 2 x 2777 x 16 / 4 in 396 + 20 in four and 436 + 31 in
+// six.)
+inline Plan plan(long problems, int outer, int inner, int finest, int causal, int slots, float traffic, bool whole) {
   Plan p;
   p.wide = outer > 32;
   p.nblk = cdiv(outer, p.wide ? 128 : 32);
   const long blocks = problems * p.nblk;
   long n = blocks >= slots ? 1 : (2 * slots + blocks - 1) / blocks, most = inner / finest < 1 ? 1 : inner / finest;
-  if (p.wide) {
+  if (whole) {
     const float load = (float)blocks / slots;
     float best = 0.f;
     long pick = 1;

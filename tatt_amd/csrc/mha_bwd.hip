@@ -320,10 +320,10 @@ __global__ __launch_bounds__(256) void mha_sum_kernel(const float* __restrict__ 
 
 // Splits of no less than 256 (2 x 1024 x 1024, 4 heads of 64: fp32 70 us against 104 with 512, bf16 39 against 44; with 128 94 and 51)
 Plan plan_dq(int B, int Lq, int Lk, int H, int Hkv, int D, int causal, int dtype) {
-  return plan((long)B * Hkv, Lq * (H / Hkv), Lk, 256, causal, slots_of(dtype == TATT_T_BF16 ? dq_waves<bf16_t>(D) : dq_waves<float>(D > 32 ? 64 : D)), traffic_of(dtype));
+  return plan((long)B * Hkv, Lq * (H / Hkv), Lk, 256, causal, slots_of(dtype == TATT_T_BF16 ? dq_waves<bf16_t>(D) : dq_waves<float>(D > 32 ? 64 : D)), traffic_of(dtype), true);
 }
 Plan plan_dkv(int B, int Lq, int Lk, int H, int Hkv, int D, int causal, int dtype) {
-  return plan((long)B * Hkv, Lk, Lq * (H / Hkv), 256, causal, slots_of(dtype == TATT_T_BF16 ? dkv_waves<bf16_t>(D) : dkv_waves<float>(D > 64 ? D : D > 32 ? 64 : D)), traffic_of(dtype));
+  return plan((long)B * Hkv, Lk, Lq * (H / Hkv), 256, causal, slots_of(dtype == TATT_T_BF16 ? dkv_waves<bf16_t>(D) : dkv_waves<float>(D > 64 ? D : D > 32 ? 64 : D)), traffic_of(dtype), Lk > 32);
 }
 
 template <typename T, int DK, int R, int SUB>

@@ -286,9 +286,12 @@ __global__ __launch_bounds__(256) void mha_fwd_join(const float* __restrict__ pa
 // A split costs its partial sums, a second launch and the workspace: with bf16 tiles, done quickly, 512 keys are worth that (8 x 8 heads of 64, one query,
 // 1000 keys: 12 us unsplit and 16 in splits of 256; 20000 keys, 32 / 8 heads of 128: 149 in splits and 447 without), with fp32 ones 128 (17 us in splits
 // of 128 and 28 of 512; one query, 4000 keys, 8 key heads of 128: 43 and 92; with two waves, below, 29).
+// Workgroups at once: of one wave and 48 KB (fp32 heads past 64, few rows) three a CU (8 x 20000 keys, 8 heads of 128, one query: 317 us in 23 splits,
+// 402 in 8).
 Plan plan_fwd(int B, int Lq, int Lk, int H, int Hkv, int D, int causal, int dtype) {
   const bool bf16 = dtype == TATT_T_BF16;
-  return plan((long)B * Hkv, Lq * (H / Hkv), Lk, bf16 ? 512 : 128, causal, slots_of(bf16 ? fwd_waves<bf16_t>(D) : fwd_waves<float>(D)), traffic_of(dtype));
+  const int rows = Lq * (H / Hkv), slots = rows > 32 ? slots_of(bf16 ? fwd_waves<bf16_t>(D) : fwd_waves<float>(D)) : !bf16 && D > 64 ? 768 : 512;
+  return plan((long)B * Hkv, rows, Lk, bf16 ? 512 : 128, causal, slots, traffic_of(dtype), rows > 32);
 }
 
 template <typename T, int DK, int WQ, int R, int WK, int SUB, int JOINT>
