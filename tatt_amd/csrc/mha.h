@@ -18,8 +18,8 @@
 // the second kind if the contraction visits the tile's rows in that order: no element changes its lane between the two products.
 // The MFMA is v_mfma_f32_32x32x16_bf16; transposed reads are ds_read_b64_tr_b16 (4 rows x 16 dimensions to 16 lanes).  fp32 tensors go through the
 // same products as three bf16 pieces of every operand (fp32 accuracy; 6 bf16 MFMAs of 8 passes against 8 fp32 ones of 16).
-// Operands are rounded to bf16 only where the tensors are bf16 (P and dS enter their second product in bf16: 2^-9 of a term, the error that the
-// stored result carries anyway); accumulation is fp32.
+// Operands that are computed, P and dS, enter their second product beside bf16 tensors as two bf16 pieces (16 significant bits: 2^-16 of a term, where
+// one piece is off by up to 2^-8 of it, as much as the rounding of the stored result); accumulation is fp32.
 #pragma once
 #include "token_types.h"
 
@@ -30,16 +30,20 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // A lane's 8 contraction places of a step, as the matrix core takes them.  bf16 tensors: the values.  fp32 tensors: three bf16 pieces of each value,
 // x = x0 + x1 + x2 exactly (3 x 8 significant bits); a product is the six terms a0 b0 + (a0 b1 + a1 b0) + (a0 b2 + a1 b1 + a2 b0), added in fp32,
-// smallest first, and what is left out is below the rounding of one fp32 product.
-template <typename T>
+// smallest first, and what is left out is below the rounding of one fp32 product.  What is computed beside bf16 tensors: two pieces, two products with
+// one reading of the other operand.
+template <typename T, int N = (sizeof(T) == 2 ? 1 : 3)>
 struct Frag {
-  static constexpr int PIECES = sizeof(T) == 2 ? 1 : 3;
+  static constexpr int PIECES = N;
   bf16x8 p[PIECES];
 };
-
 template <typename T>
-__device__ __forceinline__ f32x16 mma(const Frag<T>& a, const Frag<T>& b, f32x16 c) {
-  if constexpr (Frag<T>::PIECES == 3) {
+constexpr int COMPUTED = sizeof(T) == 2 ? 2 : 3;  // pieces of P and dS
+
+template <typename T, int N>
+__device__ __forceinline__ f32x16 mma(const Frag<T>& a, const Frag<T, N>& b, f32x16 c) {
+  if constexpr (N == 2) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[1], c, 0, 0, 0);
+  if constexpr (N == 3) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[2], c, 0, 0, 0);
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[1], c, 0, 0, 0);
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[2], b.p[0], c, 0, 0, 0);
@@ -67,22 +71,24 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t (&u)[3]) {
   u[2] = pack2(ra - low2(u[1]), rb - high2(u[1]));
 }
 
-// 8 values, v(0) .. v(7), as a fragment
-template <typename T, typename V>
-__device__ __forceinline__ Frag<T> fragment(V v) {
-  uint32_t u[Frag<T>::PIECES][4];
+// 8 values, v(0) .. v(7), as a fragment of N pieces
+template <typename T, int N, typename V>
+__device__ __forceinline__ Frag<T, N> fragment(V v) {
+  uint32_t u[N][4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    if constexpr (Frag<T>::PIECES == 3) {
+    const float a = v(2 * j), b = v(2 * j + 1);
+    if constexpr (N == 3) {
       uint32_t w[3];
-      split2(v(2 * j), v(2 * j + 1), w);
+      split2(a, b, w);
 #pragma unroll
       for (int x = 0; x < 3; ++x) u[x][j] = w[x];
     } else {
-      u[0][j] = pack2(v(2 * j), v(2 * j + 1));
+      u[0][j] = pack2(a, b);
+      if constexpr (N == 2) u[1][j] = pack2(a - low2(u[0][j]), b - high2(u[0][j]));
     }
   }
-  Frag<T> f;
+  Frag<T, N> f;
   memcpy(&f, u, sizeof(f));
   return f;
 }
@@ -91,8 +97,8 @@ constexpr int STEP = 16;  // contraction places of an MFMA step (both lane halve
 
 // accumulator registers 8 step .. 8 step + 7 as the B operand of the transposed product's step
 template <typename T>
-__device__ __forceinline__ Frag<T> pack_step(const f32x16& c, int step) {
-  return fragment<T>([&](int j) { return c[8 * step + j]; });
+__device__ __forceinline__ Frag<T, COMPUTED<T>> pack_step(const f32x16& c, int step) {
+  return fragment<T, COMPUTED<T>>([&](int j) { return c[8 * step + j]; });
 }
 
 // waves a SIMD that the registers are shared out for.  Two (256 registers each) unless what a wave has to hold -- the fragments of its rows, the
@@ -249,7 +255,7 @@ struct RowFrags {
       if constexpr (sizeof(T) == 2)
         memcpy(&f[s], t, 16);
       else
-        f[s] = fragment<T>([&](int j) { return t[j]; });
+        f[s] = fragment<T, Frag<T>::PIECES>([&](int j) { return t[j]; });
     }
   }
   // the product with another row

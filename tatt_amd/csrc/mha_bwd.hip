@@ -115,7 +115,7 @@ __global__ __launch_bounds__(64 * WQ, dq_waves<T>(DK)) void mha_dq_kernel(MhaArg
           for (int i = 0; i < 16; ++i) sc[r][i] = see >> acc_row(i) & 1 ? sc[r][i] : 0.f;
         }
       }
-      Frag<T> p[R][TS];
+      Frag<T, COMPUTED<T>> p[R][TS];
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll

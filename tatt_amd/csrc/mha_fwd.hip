@@ -138,7 +138,7 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
       }
 #pragma unroll
       for (int s = 0; s < JOINT; ++s) {
-        Frag<T> p[R][TS];
+        Frag<T, COMPUTED<T>> p[R][TS];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
 #pragma unroll
