@@ -57,6 +57,11 @@ def _no_tangent(what, *tensors):
         raise NotImplementedError(f"tatt_amd {what}: no forward-mode derivatives")      # the result would have none, as if they were zero
 
 
+def _constant(what, *values):
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in values):
+        raise NotImplementedError(f"tatt_amd {what}: no gradient of a value that requires one")     # autograd would leave it None
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -153,7 +158,8 @@ class _LayerNormFn(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
     """LayerNorm over the last dimension of x (float32 or bfloat16; weight and bias float32 or None), any width.  With a residual:
     -> (LayerNorm(sum), sum), sum = x + residual rounded to x's type, in one pass."""
-    _no_tangent("layer_norm", x, residual, weight, bias)
+    _no_tangent("layer_norm", x, residual, weight, bias, eps)
+    _constant("layer_norm: eps", eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight, bias)):
         return _LayerNormFn.apply(x, residual, weight, bias, eps)
     y, s, _ = layer_norm_forward(x, weight, bias, eps, residual, need_stat=False)
@@ -218,8 +224,10 @@ class _RotaryFn(torch.autograd.Function):
 def rotary(q, k, positions, freqs, sections, interleaved=False):
     """Rotary positions over several axes.  q [B, L, H, D] and k [B, L, Hk, D] or None (float32 or bfloat16, any strides); positions
     [L, axes] or [B, L, axes], int64, int32 or float32; the first sections[0] dimensions of each head turn by positions[..., 0], the next
-    sections[1] by positions[..., 1] and so on, the rest passes through; freqs = rotary_frequencies(sections).  -> (q', k'), or q' if k is None."""
+    sections[1] by positions[..., 1] and so on, the rest passes through; freqs = rotary_frequencies(sections).  Positions and freqs have no
+    gradient (refused if they require one).  -> (q', k'), or q' if k is None."""
     _no_tangent("rotary", q, k, positions, freqs)
+    _constant("rotary: positions and freqs", positions, freqs)
     sections = tuple(int(s) for s in sections)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _RotaryFn.apply(q, k, positions, freqs, sections, bool(interleaved))
@@ -328,6 +336,7 @@ def attention(q, k, v, key_padding_mask=None, causal=False, scale=None):
     causality hides it included (0 times it).  float32 keeps its accuracy for magnitudes of 2^-100 to 2^127, scores (scaled) for magnitudes below
     2^28, past which a row may be NaN; the gradients' probabilities are off by 2^-24 of the score, relative to themselves."""
     _no_tangent("attention", q, k, v, scale)
+    _constant("attention: scale", scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _AttentionFn.apply(q, k, v, key_padding_mask, causal, scale)
     return attention_forward(q, k, v, key_padding_mask, causal, scale, need_saved=False)[0]

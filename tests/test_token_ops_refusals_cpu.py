@@ -23,3 +23,23 @@ def test_forward_mode_derivatives_are_refused(op, at):
             call(*args)
     with pytest.raises(RuntimeError, match="GPU only"):      # not refused for it any more
         call(*(torch.randn(*s) for s in shapes))
+
+
+@pytest.mark.parametrize("queries_too", [False, True])
+@pytest.mark.parametrize("op,what", [("rotary", "positions"), ("rotary", "freqs"), ("attention", "scale"), ("layer_norm", "eps")])
+def test_values_without_a_gradient_are_refused_where_they_require_one(op, what, queries_too):
+    """autograd would leave the gradient None, or the whole result without one."""
+    call, shapes = CALLS[op]
+    args = [torch.randn(*s) for s in shapes]
+    args[0].requires_grad_(queries_too)
+    value = torch.tensor(0.5, requires_grad=True)
+    if op == "rotary":
+        args[{"positions": 2, "freqs": 3}[what]].requires_grad_()
+    elif op == "attention":
+        call = lambda q, k, v: T.attention(q, k, v, scale=value)    # noqa: E731
+    else:
+        call = lambda x, *_: T.layer_norm(x, eps=value)    # noqa: E731
+    with pytest.raises(NotImplementedError, match=f"tatt_amd {op}: .*{what}.*no gradient"):
+        call(*args)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):      # nothing is lost here
+        call(*args)
