@@ -533,7 +533,13 @@ inline Plan plan(long problems, int outer, int inner, int finest, int causal, in
 inline int slots_of(int waves) { return waves == 1 ? 256 : 512; }
 inline float traffic_of(int dtype) { return dtype == TATT_T_BF16 ? 400.f : 80.f; }
 
-inline bool sane(int B, int Lq, int Lk, int H, int Hkv, int D) { return B > 0 && Lq > 0 && Lk > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && D > 0; }
+// fewer than 2^30 rows of a tensor, factor by factor: three of 31 bits overflow 64
+inline bool countable(int B, int H, int L) { return (long)B * H < 1L << 30 && (long)B * H * L < 1L << 30; }
+
+// what the entry points take, and the workspace queries answer (the plans' own products stay within 31 bits)
+inline bool sane(int B, int Lq, int Lk, int H, int Hkv, int D) {
+  return B > 0 && Lq > 0 && Lk > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && H / Hkv <= 1 << 16 && D > 0 && D <= 128 && countable(B, H, Lq) && countable(B, Hkv, Lk);
+}
 
 // 16-byte rows, and a tile of 128 of them (G heads of 128 / G tokens) within the 31-bit offsets of a buffer load
 inline bool reachable(const void* p, const long* s, int size, int G) {
@@ -552,7 +558,7 @@ inline int fill(MhaArgs& a, const char* who, const void* q, const void* k, const
   TATT_CHECK_ARG(D > 0 && D <= 128, "%s: built for heads of 1 to 128, got %d", who, D);
   TATT_CHECK_ARG(dtype == TATT_T_F32 || dtype == TATT_T_BF16, "%s: unknown element type %d", who, dtype);
   TATT_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "%s: the workspace is not 16-byte aligned", who);
-  TATT_CHECK_ARG((long)B * H * Lq < (1L << 30) && (long)B * Hkv * Lk < (1L << 30), "%s: 2^30 rows or more", who);
+  TATT_CHECK_ARG(countable(B, H, Lq) && countable(B, Hkv, Lk), "%s: 2^30 rows or more", who);
   a.q = q, a.k = k, a.v = v, a.out = out, a.dout = dout, a.mask = mask;
   a.mask_sb = mask ? mask_strides[0] : 0, a.mask_sl = mask ? mask_strides[1] : 0;
   for (int i = 0; i < 3; ++i) a.qs[i] = strides[i], a.ks[i] = strides[3 + i], a.vs[i] = strides[6 + i];

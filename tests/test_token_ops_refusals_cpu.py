@@ -1,8 +1,13 @@
 """Calls that the token operators would answer wrongly and refuse instead, checked without a GPU: every refusal comes before any launch."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
+from tatt_amd import lib as tl
 from tatt_amd.model import token_ops as T
 
 CALLS = {  # operator -> (its call, shapes of its tensors)
@@ -43,3 +48,29 @@ def test_values_without_a_gradient_are_refused_where_they_require_one(op, what, 
         call(*args)
     with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):      # nothing is lost here
         call(*args)
+
+
+REFUSED = [  # B, Lq, Lk, H, Hkv, D: rows past 2^30, products past 31 and 64 bits, heads, widths
+    (1, 1 << 16, 1, 1 << 16, 1, 8), (1, 1 << 15, 40, 1 << 16, 1, 8), (1, (1 << 31) - 1, 5, 2, 1, 8), (1, 1, (1 << 31) - 1, 1, 1, 8), (1 << 22, 1 << 21, 1, 1 << 21, 1 << 21, 8),
+    (1 << 22, 1, 1 << 21, 1 << 21, 1 << 21, 8), (1, 1, 1, 1 << 17, 1, 8), (1, 1, 1, 1, 1, 129), (1, 1, 1, 3, 2, 8), (0, 1, 1, 1, 1, 8), (1, -1, 1, 1, 1, 8)]
+
+
+def test_attention_workspace_queries_of_what_is_refused():
+    """0, from a process that lives on: row counts past 31 bits ended it with a division by zero."""
+    ask = "from tatt_amd.lib import lib; c = lib().cdll\n" + "\n".join(
+        f"print(c.tatt_mha_{way}_workspace{(*dims, dtype)}, flush=True)" for dims in REFUSED for way in ("fwd", "bwd") for dtype in (0, 1))
+    child = subprocess.run([sys.executable, "-c", ask], capture_output=True, text=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), timeout=300)
+    assert child.returncode == 0, (child.returncode, len(child.stdout.split()))
+    assert child.stdout.split() == ["0"] * 4 * len(REFUSED)
+    assert tl.lib().mha_bwd_workspace(2, 3, 5, 4, 2, 16, 0) >= 2 * 3 * 4       # what is taken has one
+
+
+@pytest.mark.parametrize("dims", [d for d in REFUSED if min(d) > 0], ids=lambda d: "x".join(map(str, d)))
+def test_attention_entry_points_refuse_the_same(dims):
+    B, Lq, Lk, H, Hkv, D = dims
+    p = 4096     # a stand-in for a device pointer: refused before it is used
+    strides = (tl.ctypes.c_long * 15)()
+    with pytest.raises(RuntimeError, match="tatt_mha_fwd: "):
+        tl.lib().mha_fwd(p, p, p, strides, None, None, p, None, None, B, Lq, Lk, H, Hkv, D, 1.0, 0, 0, p, None)
+    with pytest.raises(RuntimeError, match="tatt_mha_bwd: "):
+        tl.lib().mha_bwd(p, p, p, strides, None, None, p, None, p, p, p, p, p, B, Lq, Lk, H, Hkv, D, 1.0, 0, 0, p, None)
