@@ -52,6 +52,11 @@ def _first_order(what):
         raise NotImplementedError(f"tatt_amd {what}: no gradient of the gradient")
 
 
+def _int(what, *sizes):
+    if any(n >> 31 for n in sizes):
+        raise RuntimeError(f"tatt_amd {what}: a dimension of 2^31 or more, got {sizes}")      # the C ABI would get its low 32 bits
+
+
 def _no_tangent(what, *tensors):
     if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"tatt_amd {what}: no forward-mode derivatives")      # the result would have none, as if they were zero
@@ -101,6 +106,7 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None, need_
         raise RuntimeError(f"tatt_amd layer_norm: the residual has the shape of x, got {tuple(residual.shape)} and {tuple(x.shape)}")
     _parameters("layer_norm", x, weight, bias)
     C = x.shape[-1]
+    _int("layer_norm", C)
     R = x.numel() // C
     y = _like(x)
     s = _like(x) if residual is not None else x
@@ -119,6 +125,7 @@ def layer_norm_backward(dy, s, weight, stat, dsum=None, need_params=True):
     dtype = _check("layer_norm", s, dy, dsum)
     _parameters("layer_norm", s, weight, None)
     C = s.shape[-1]
+    _int("layer_norm", C)
     R = s.numel() // C
     if dy.shape != s.shape or (dsum is not None and dsum.shape != s.shape) or stat.shape != (R, 2) or stat.dtype != torch.float32 or stat.device != s.device or not stat.is_contiguous():
         raise RuntimeError("tatt_amd layer_norm_backward: dy and dsum have the shape of the sum, stat is layer_norm_forward's")
@@ -179,6 +186,7 @@ def rotate(q, k, positions, freqs, sections, interleaved=False, inverse=False):
     if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
         raise RuntimeError("tatt_amd rotary: q [B, L, H, D] and k [B, L, Hk, D] expected")
     B, L, H, D = q.shape
+    _int("rotary", B, H, D, 0 if k is None else k.shape[2])
     if not 1 <= n <= 4 or min(sections) <= 0 or any(s & 1 for s in sections) or width > D:
         raise RuntimeError(f"tatt_amd rotary: one to four positive even sections of at most {D} dimensions together, got {tuple(sections)}")
     kind, shape, device = _POS_TYPES.get(positions.dtype), positions.shape, q.device
@@ -242,6 +250,7 @@ def _attention_args(q, k, v, mask, scale):
         raise RuntimeError(f"tatt_amd attention: q [B, Lq, H, D] and k, v [B, Lk, Hk, D] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     B, Lq, H, D = q.shape
     Lk, Hk = k.shape[1:3]
+    _int("attention", B, Lq, Lk, H, Hk)
     if not 0 < D <= 128:
         raise NotImplementedError(f"tatt_amd attention: heads of 1 to 128 dimensions, got {D}")
     if Hk == 0 or H == 0 or H % Hk:

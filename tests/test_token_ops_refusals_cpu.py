@@ -74,3 +74,28 @@ def test_attention_entry_points_refuse_the_same(dims):
         tl.lib().mha_fwd(p, p, p, strides, None, None, p, None, None, B, Lq, Lk, H, Hkv, D, 1.0, 0, 0, p, None)
     with pytest.raises(RuntimeError, match="tatt_mha_bwd: "):
         tl.lib().mha_bwd(p, p, p, strides, None, None, p, None, p, p, p, p, p, B, Lq, Lk, H, Hkv, D, 1.0, 0, 0, p, None)
+
+
+FAR = (1 << 32) + 1     # its low 32 bits: 1
+
+
+def meta(*shape):
+    return torch.empty(1, dtype=torch.bfloat16, device="meta").expand(shape)
+
+
+@pytest.mark.parametrize("op,call", [
+    ("layer_norm", lambda: T.layer_norm(meta(1, FAR + 7))), ("layer_norm", lambda: T.layer_norm_backward(meta(1, FAR + 7), meta(1, FAR + 7), None, torch.empty(1, 2, device="meta"))),
+    ("rotary", lambda: T.rotate(meta(FAR, 1, 1, 2), None, torch.empty(1, 1, device="meta"), torch.empty(1, dtype=torch.float64, device="meta"), (2,))),
+    ("rotary", lambda: T.rotate(meta(1, 1, 1, 2), meta(1, 1, FAR, 2), torch.empty(1, 1, device="meta"), torch.empty(1, dtype=torch.float64, device="meta"), (2,))),
+    ("rotary", lambda: T.rotate(meta(1, 1, 1, FAR), None, torch.empty(1, 1, device="meta"), torch.empty(1, dtype=torch.float64, device="meta"), (2,))),
+    ("attention", lambda: T.attention_forward(meta(FAR, 1, 1, 8), meta(FAR, 1, 1, 8), meta(FAR, 1, 1, 8))),
+    ("attention", lambda: T.attention_forward(meta(1, 1, 1, 8), meta(1, FAR, 1, 8), meta(1, FAR, 1, 8))),
+    ("attention", lambda: T.attention_forward(meta(1, FAR, 1, 8), meta(1, 1, 1, 8), meta(1, 1, 1, 8))),
+    ("attention", lambda: T.attention_forward(meta(1, 1, FAR, 8), meta(1, 1, 1, 8), meta(1, 1, 1, 8)))])
+def test_dimensions_past_31_bits_are_refused(op, call, monkeypatch):
+    """The C ABI's int would take the low 32 bits, and the call would leave all but the first rows unwritten.  Tensors without memory, and a stand-in for the
+    launch: a call that gets that far is not refused."""
+    monkeypatch.setattr(T, "_check", lambda what, t0, *tensors: 1)
+    monkeypatch.setattr(T, "_call", lambda name, device, *args: pytest.fail(f"{name} would be launched"))
+    with pytest.raises(RuntimeError, match=f"tatt_amd {op}: a dimension of 2.31"):
+        call()
