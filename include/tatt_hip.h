@@ -368,7 +368,7 @@ int tatt_clip_adam(float* p, const float* g, float* m, float* v, long n, float l
  * void* tensors are of that type; strides count elements; `strides` arguments are HOST arrays, read during the call.  Outputs and
  * workspaces overlap nothing else; two calls in flight need a workspace each.  No atomics: results are bit-reproducible.
  *
- * LayerNorm over C columns (nn.LayerNorm at model/transformer_v2.py:478-482, :827-831, of any width), optionally with the residual sum in front:
+ * LayerNorm over C < 2^27 columns (nn.LayerNorm at model/transformer_v2.py:478-482, :827-831, of any width), optionally with the residual sum in front:
  *   s = x + res (stored to sum, contiguous, rounded to the type; res = NULL: s = x), y = (s - mu) rstd gamma + beta (NULL: 1 / 0),
  *   stat[row] = (mu, rstd) for the backward call (may be NULL).  ld* = elements between rows; y, sum, dx contiguous.
  * tatt_layernorm_bwd: dx = d loss / d s (+ dsum, the gradient that reaches s by other ways; NULL: none), dgamma, dbeta written (each

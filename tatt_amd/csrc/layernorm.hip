@@ -307,16 +307,16 @@ __global__ __launch_bounds__(256) void layernorm_dx_wide(const T* __restrict__ s
 template <typename T>
 __global__ __launch_bounds__(256) void layernorm_params_wide(const T* __restrict__ s, long lds, const T* __restrict__ dy, long lddy,
                                                              const float* __restrict__ stat, float* __restrict__ partial, long rows, int C) {
-  const int c = blockIdx.y * 256 + threadIdx.x;
-  if (c >= C) return;
-  float dg = 0.f, db = 0.f;
-  for (long r = blockIdx.x; r < rows; r += gridDim.x) {
-    const float d = to_f32(dy[r * lddy + c]);
-    dg += d * ((to_f32(s[r * lds + c]) - stat[2 * r]) * stat[2 * r + 1]);
-    db += d;
+  for (int c = blockIdx.y * 256 + threadIdx.x; c < C; c += gridDim.y * 256) {
+    float dg = 0.f, db = 0.f;
+    for (long r = blockIdx.x; r < rows; r += gridDim.x) {
+      const float d = to_f32(dy[r * lddy + c]);
+      dg += d * ((to_f32(s[r * lds + c]) - stat[2 * r]) * stat[2 * r + 1]);
+      db += d;
+    }
+    partial[(blockIdx.x * 2L) * C + c] = dg;
+    partial[(blockIdx.x * 2L + 1) * C + c] = db;
   }
-  partial[(blockIdx.x * 2L) * C + c] = dg;
-  partial[(blockIdx.x * 2L + 1) * C + c] = db;
 }
 
 // partial[block][2][C] -> dgamma, dbeta, in block order
@@ -384,6 +384,8 @@ int bwd_blocks(long rows, int C, int dtype) {
 }
 
 constexpr long MAX_GRID = 1 << 16;  // workgroups of the forward pass: more rows go round
+constexpr int MAX_GRID_Y = 65535;   // and of the grid's second axis: more columns go round
+constexpr int MAX_COLUMNS = 1 << 27;  // a column and the loops' steps past it stay within an int, 16 columns a workgroup within the grid
 
 bool lined_up(const void* p, long ld, int size) { return !p || (((uintptr_t)p & 15) == 0 && ld * size % 16 == 0); }
 
@@ -394,6 +396,7 @@ extern "C" {
 int tatt_layernorm_fwd(const void* x, long ldx, const void* res, long ldr, const float* gamma, const float* beta, void* sum, void* y,
                        float* stat, long rows, int C, float eps, int dtype, hipStream_t st) {
   TATT_CHECK_ARG(x && y && rows > 0 && C > 0 && (ldx >= C || ldx == 0) && (!res || (sum && (ldr >= C || ldr == 0))), "tatt_layernorm_fwd: bad arguments (rows %ld, C %d)", rows, C);
+  TATT_CHECK_ARG(C < MAX_COLUMNS, "tatt_layernorm_fwd: rows of 2^27 elements or more");
   TATT_CHECK_ARG(dtype == TATT_T_F32 || dtype == TATT_T_BF16, "tatt_layernorm_fwd: unknown element type %d", dtype);
   TATT_CHECK_ARG(((uintptr_t)stat & 7) == 0, "tatt_layernorm_fwd: stat is not 8-byte aligned");
   const int size = dtype == TATT_T_BF16 ? 2 : 4;
@@ -412,13 +415,14 @@ int tatt_layernorm_fwd(const void* x, long ldx, const void* res, long ldr, const
   return TATT_OK;
 }
 
-size_t tatt_layernorm_workspace(long rows, int C, int dtype) { return rows > 0 && C > 0 ? (size_t)bwd_blocks(rows, C, dtype) * 2 * C : 0; }
+size_t tatt_layernorm_workspace(long rows, int C, int dtype) { return rows > 0 && C > 0 && C < MAX_COLUMNS ? (size_t)bwd_blocks(rows, C, dtype) * 2 * C : 0; }
 
 int tatt_layernorm_bwd(const void* s, long lds, const void* dy, long lddy, const void* dsum, long ldds, const float* gamma,
                        const float* stat, void* dx, float* dgamma, float* dbeta, long rows, int C, int dtype, float* workspace,
                        hipStream_t st) {
   TATT_CHECK_ARG(s && dy && stat && dx && rows > 0 && C > 0 && (lds >= C || lds == 0) && (lddy >= C || lddy == 0) && (!dsum || ldds >= C || ldds == 0),
                  "tatt_layernorm_bwd: bad arguments (rows %ld, C %d)", rows, C);
+  TATT_CHECK_ARG(C < MAX_COLUMNS, "tatt_layernorm_bwd: rows of 2^27 elements or more");
   TATT_CHECK_ARG(dtype == TATT_T_F32 || dtype == TATT_T_BF16, "tatt_layernorm_bwd: unknown element type %d", dtype);
   TATT_CHECK_ARG(workspace || (!dgamma && !dbeta), "tatt_layernorm_bwd: parameter gradients need tatt_layernorm_workspace floats");
   TATT_CHECK_ARG(((uintptr_t)stat & 7) == 0, "tatt_layernorm_bwd: stat is not 8-byte aligned");
@@ -431,7 +435,7 @@ int tatt_layernorm_bwd(const void* s, long lds, const void* dy, long lddy, const
         hipLaunchKernelGGL(layernorm_dx_wide<T>, dim3((unsigned)((rows + 3) / 4 < MAX_GRID ? (rows + 3) / 4 : MAX_GRID)), dim3(256), 0, st, (const T*)s, lds,
                            (const T*)dy, lddy, (const T*)dsum, ldds, gamma, stat, (T*)dx, rows, C);
         if (params)
-          hipLaunchKernelGGL(layernorm_params_wide<T>, dim3(n, cdiv(C, 256)), dim3(256), 0, st, (const T*)s, lds, (const T*)dy, lddy, stat, workspace, rows, C);
+          hipLaunchKernelGGL(layernorm_params_wide<T>, dim3(n, cdiv(C, 256) < MAX_GRID_Y ? cdiv(C, 256) : MAX_GRID_Y), dim3(256), 0, st, (const T*)s, lds, (const T*)dy, lddy, stat, workspace, rows, C);
       } else TATT_DISPATCH_HELD(h, launch_bwd<T, TPR, NV>(vec, params, n, st, (const T*)s, lds, (const T*)dy, lddy, (const T*)dsum, ldds, gamma, stat, (T*)dx,
                                                           workspace, rows, C););
   );

@@ -163,7 +163,7 @@ class _LayerNormFn(torch.autograd.Function):
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
-    """LayerNorm over the last dimension of x (float32 or bfloat16; weight and bias float32 or None), any width.  With a residual:
+    """LayerNorm over the last dimension of x (float32 or bfloat16; weight and bias float32 or None), of any width below 2^27.  With a residual:
     -> (LayerNorm(sum), sum), sum = x + residual rounded to x's type, in one pass."""
     _no_tangent("layer_norm", x, residual, weight, bias, eps)
     _constant("layer_norm: eps", eps)

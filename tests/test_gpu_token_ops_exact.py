@@ -34,3 +34,21 @@ def test_attention_in_bf16_rounds_only_what_it_stores(shape, kind, causal):
     B, Lq, Lk, H, Hk, D = shape
     q, k, v = heads("tokens", *shape, BF16, 21)
     attention_in_bounds(q, k, v, rnd(B, Lq, H, D, seed=9, dtype=BF16), key_mask(kind, B, Lk), causal, D ** -0.5, 2.0 ** -16 + 2.0 ** -15)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+def test_layer_norm_of_rows_past_the_grid(dtype):
+    """More columns than 65535 workgroups of 256 take at once.  Values of 1 and -1 in turn: mean 0 and variance 1 without rounding, and every result one product
+    of 1 / sqrt(1 + eps), which fp32 holds to a few roundings."""
+    R, C = 3, 65535 * 256 + 4098
+    x = torch.ones(R, C, dtype=dtype, device="cuda")
+    x[:, ::2] = -1
+    dy = (torch.arange(R * C, device="cuda") % 7 - 3).view(R, C).to(dtype)
+    y, s, stat = T.layer_norm_forward(x)
+    dx, dw, db = T.layer_norm_backward(dy, s, None, stat)
+    r = (1 + 1e-5) ** -0.5
+    assert (y.float() - x.float() * r).abs().max() <= STORED[dtype] + 2.0 ** -21
+    g = dy.double()
+    assert (dw.double() - (g * x.double()).sum(0) * r).abs().max() <= 9 * 2.0 ** -21 and torch.equal(db.double(), g.sum(0))
+    want = r * (g - g.mean(1, keepdim=True) - x.double() * r * (g * x.double() * r).mean(1, keepdim=True))
+    assert ((dx.double() - want).abs() <= STORED[dtype] * want.abs() + 2.0 ** -18).all()

@@ -99,3 +99,13 @@ def test_dimensions_past_31_bits_are_refused(op, call, monkeypatch):
     monkeypatch.setattr(T, "_call", lambda name, device, *args: pytest.fail(f"{name} would be launched"))
     with pytest.raises(RuntimeError, match=f"tatt_amd {op}: a dimension of 2.31"):
         call()
+
+
+@pytest.mark.parametrize("C", [1 << 27, (1 << 31) - 1])
+def test_layernorm_refuses_rows_past_its_loops(C):
+    p = 4096     # a stand-in for a device pointer: refused before it is used
+    with pytest.raises(RuntimeError, match="2.27 elements"):
+        tl.lib().layernorm_fwd(p, C, None, 0, None, None, None, p, None, 1, C, 1e-5, 0, None)
+    with pytest.raises(RuntimeError, match="2.27 elements"):
+        tl.lib().layernorm_bwd(p, C, p, C, None, 0, None, p, p, None, None, 1, C, 0, None, None)
+    assert tl.lib().layernorm_workspace(1, C, 0) == 0
