@@ -3,7 +3,7 @@
 //   y = (s - mu) rstd * gamma + beta          stat[row] = (mu, rstd)
 //   g = dy * gamma,  xhat = (s - mu) rstd,  ds = rstd (g - mean(g) - xhat mean(g xhat)) (+ dsum)
 //   dgamma = sum over rows of dy * xhat,  dbeta = sum over rows of dy
-// Statistics, sums and parameter gradients are fp32 whatever the tensors' type.
+// Statistics, sums and parameter gradients are fp32 whatever the tensors' type (sums over the rows of several threads 64 bits).
 // Bound by memory, so every tensor is touched once: a row lives in the registers of its TPR threads as NV 16-byte chunks each (mean, then the
 // variance of the differences: two passes over registers, no difference of squares), and the backward pass takes dx and the sums over
 // rows from the same registers, its threads keeping their columns from row to row.
@@ -228,10 +228,10 @@ __global__ __launch_bounds__(block_of(TPR)) void layernorm_bwd_kernel(const T* _
           __syncthreads();
           for (int i = threadIdx.x; i < TPR * E; i += 256) {
             const int c = (n * TPR + i / E) * E + i % E;
-            float v = 0.f;
+            double v = 0.;
 #pragma unroll
             for (int r = 0; r < PER; ++r) v += cols[(i % E) * 256 + r * TPR + i / E];
-            if (c < C) p[which * C + c] = v;
+            if (c < C) p[which * C + c] = (float)v;
           }
         } else {
 #pragma unroll
@@ -319,14 +319,33 @@ __global__ __launch_bounds__(256) void layernorm_params_wide(const T* __restrict
   }
 }
 
-// partial[block][2][C] -> dgamma, dbeta, in block order
+// partial[block][2][C] -> dgamma, dbeta, in block order: 16 columns of a workgroup by 16 threads each, four loads of a thread in flight.  Sums over
+// rows are fp32 only within a thread; past it their roundings would be most of the error (65536 x 64: 1.5e-7 of the result, 7e-8 so).
 __global__ __launch_bounds__(256) void layernorm_params_final(const float* __restrict__ partial, int nblk, int C,
                                                               float* __restrict__ dgamma, float* __restrict__ dbeta) {
-  __shared__ float red[256];
+  __shared__ double red[256];
   const int c = blockIdx.x * 16 + (threadIdx.x & 15);
   float* dst = blockIdx.y ? dbeta : dgamma;
-  const float v = block16_colsum(partial + (long)blockIdx.y * C, nblk, 2L * C, c, c < C, red);
-  if (threadIdx.x < 16 && c < C && dst) dst[c] = v;
+  if (!dst) return;
+  const float* p = partial + (long)blockIdx.y * C + c;
+  double s[4] = {0., 0., 0., 0.};
+  int b = threadIdx.x >> 4;
+  if (c < C) {
+    for (; b + 48 < nblk; b += 64) {
+      float t[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = p[(b + 16 * i) * 2L * C];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] += t[i];
+    }
+    for (; b < nblk; b += 16) s[0] += p[b * 2L * C];
+  }
+  red[threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  if (threadIdx.x >= 16 || c >= C) return;
+  double v = 0.;
+  for (int j = 0; j < 16; ++j) v += red[16 * j + threadIdx.x];
+  dst[c] = (float)v;
 }
 
 // how a row of C elements is held: threads of a row and 16-byte chunks of a thread (0: by none, the wide kernels)

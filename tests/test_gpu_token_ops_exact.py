@@ -52,3 +52,32 @@ def test_layer_norm_of_rows_past_the_grid(dtype):
     assert (dw.double() - (g * x.double()).sum(0) * r).abs().max() <= 9 * 2.0 ** -21 and torch.equal(db.double(), g.sum(0))
     want = r * (g - g.mean(1, keepdim=True) - x.double() * r * (g * x.double() * r).mean(1, keepdim=True))
     assert ((dx.double() - want).abs() <= STORED[dtype] * want.abs() + 2.0 ** -18).all()
+
+
+@pytest.mark.parametrize("C,n", [(64, 4), (200, 16)])
+def test_layer_norm_parameter_sums(C, n):
+    """65536 rows, n to a thread.  A rounding is uniform over half a step: e = 2^-24 / sqrt(3) / 1.4 = 2.5e-8 of its value in the root mean square.  Relative to the
+    sum of all terms: xhat's two roundings e each and rstd's, uniform over a whole step as rsqrt's may be, 2 e, with half of its argument's: 2.5 e.  A thread's k-th
+    addition is off by e of a sum of k random terms, sqrt(k) of one: sqrt(sum of k / n) = sqrt((n + 1) / 2) e, 1.6 e and 2.9 e.  A workgroup's partial sum and the result
+    e each: 3.3 e and 4.1 e.  The sizes of partial sums are those of a random walk, whose spread moves that by up to a quarter."""
+    x, w, dy = rnd(65536, C, seed=31, scale=1.5), rnd(C, seed=32) * 0.2 + 1, rnd(65536, C, seed=33)
+    _, s, stat = T.layer_norm_forward(x, w, None)
+    _, dw, db = T.layer_norm_backward(dy, s, w, stat)
+    x64, g = x.double(), dy.double()
+    var, mean = torch.var_mean(x64, dim=1, correction=0, keepdim=True)
+    most = 1.25 * 2.5e-8 * (2.5 ** 2 + (n + 1) / 2 + 2) ** 0.5
+    for got, ref in ((dw, (g * (x64 - mean) / torch.sqrt(var + 1e-5)).sum(0)), (db, g.sum(0))):
+        off = float((got.double() - ref).norm() / ref.norm())
+        assert off <= most, off
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("C", [8, 64, 200, 1024, 4096, 20001])
+def test_layer_norm_bias_gradient_of_whole_numbers(C, dtype):
+    """Whole numbers below 2^18, at most 64 rows of them to a workgroup: its sums stay below 2^24 and need no rounding, and the sum of all, 2^31 or so, is
+    rounded once.  (Summed in fp32 the workgroups' sums would be rounded again and again.)"""
+    R, g = 16384 if C > 1024 else 65536, torch.Generator(device="cuda").manual_seed(C)
+    dy = (torch.randint(0, 256, (R, C), generator=g, device="cuda") << torch.randint(0, 11, (R, C), generator=g, device="cuda")).to(dtype)
+    s = torch.ones(1, C, dtype=dtype, device="cuda").expand(R, C)
+    _, _, db = T.layer_norm_backward(dy, s, None, torch.zeros(R, 2, device="cuda"))
+    assert torch.equal(db, dy.double().sum(0).float())
