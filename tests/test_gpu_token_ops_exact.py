@@ -1,5 +1,7 @@
 """How exact the token operators are, in closer bounds than those of test_gpu_token_ops.py, which allow for every operand of a product in the
 tensors' type."""
+import math
+
 import pytest
 import torch
 
@@ -34,6 +36,36 @@ def test_attention_in_bf16_rounds_only_what_it_stores(shape, kind, causal):
     B, Lq, Lk, H, Hk, D = shape
     q, k, v = heads("tokens", *shape, BF16, 21)
     attention_in_bounds(q, k, v, rnd(B, Lq, H, D, seed=9, dtype=BF16), key_mask(kind, B, Lk), causal, D ** -0.5, 2.0 ** -16 + 2.0 ** -15)
+
+
+def plain_fp32(q, k, v, do, scale):
+    """out, dq, dk and dv by torch's fp32 products."""
+    q, k, v, do = (t.transpose(1, 2).contiguous() for t in (q, k, v, do))
+    p = torch.softmax(q @ k.transpose(2, 3).contiguous() * scale, -1)
+    out = p @ v
+    ds = p * (do @ v.transpose(2, 3).contiguous() - (do * out).sum(-1, keepdim=True)) * scale
+    return [t.transpose(1, 2) for t in (out, ds @ k, ds.transpose(2, 3).contiguous() @ q, p.transpose(2, 3).contiguous() @ do)]
+
+
+@pytest.mark.parametrize("scale", [None, 0.3])
+@pytest.mark.parametrize("shape", [(4, 26, 26, 4, 4, 16), (4, 64, 40, 4, 4, 64), (2, 100, 300, 4, 4, 128), (2, 33, 1000, 2, 2, 96), (1, 1024, 1024, 4, 4, 64), (2, 300, 20, 2, 2, 32)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_attention_in_fp32_is_as_exact_as_plain_fp32(shape, scale):
+    """In the norm.  Emulated, the six products of three pieces are at 0.4 to 0.6 of the plain form's error and any five of them at three times it or more
+    (test_token_ops_pieces_cpu.py): 1.25 is between.  The gradients take P from the stored lse, base 2 and rounded to fp32: uniform over half a step, 2^-24 of the
+    power of two above it / sqrt(3), which is ln 2 times that of a row's P and, the rows' roundings being independent, of a gradient (1000 keys: 1.9e-7)."""
+    B, Lq, Lk, H, Hk, D = shape
+    scale = D ** -0.5 if scale is None else scale
+    q, k, v = heads("tokens", *shape, F32, 22)
+    do = rnd(B, Lq, H, D, seed=9)
+    ref = attention_64(q, k, v, do, None, False, scale)
+    out, saved = T.attention_forward(q, k, v, scale=scale)
+    own = (out, *T.attention_backward(do, q, k, v, out, saved, scale=scale))
+    of_lse = 2.0 ** (math.ceil(math.log2(float(ref["lse"].abs().max()) / math.log(2.0))) - 24) * math.log(2.0) / math.sqrt(3.0)
+    for name, a, b in zip(("out", "dq", "dk", "dv"), own, plain_fp32(q, k, v, do, scale)):
+        value = ref[name][0]
+        a, b = (float((t.double().cpu() - value).norm() / value.norm()) for t in (a, b))
+        assert a <= 1.25 * b + (0.0 if name == "out" else of_lse), (name, a, b, of_lse)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
