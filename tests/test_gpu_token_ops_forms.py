@@ -2,8 +2,10 @@
 has lanes.  The conditions are those of the launch plans (mha_fwd.hip, mha_bwd.hip, plan() in mha.h) and are asserted, so that a case does not leave
 its kernel behind when a plan changes."""
 import pytest
+import torch
 
 from tatt_amd.lib import lib
+from tatt_amd.model import token_ops as T
 
 from .test_gpu_token_ops import BF16, F32, check_attention, heads, key_mask, rnd
 from .test_gpu_token_ops_exact import attention_in_bounds
@@ -61,3 +63,52 @@ def test_more_splits_than_lanes(shape, dtype, kind):
     """The join takes the splits 64 at a time."""
     assert splits(*shape, dtype) > 64
     both_bounds(shape, dtype, kind, False)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("shape,causal", [((3, 70, 333, 4, 2, 64), False), ((3, 300, 300, 2, 2, 32), True), ((3, 1, 900, 8, 2, 128), False)], ids=str)
+def test_masks_of_any_strides(shape, causal, dtype):
+    B, Lq, Lk, H, Hk, D = shape
+    q, k, v = heads("tokens", *shape, dtype, 24)
+    do, hidden = rnd(B, Lq, H, D, seed=9, dtype=dtype), key_mask("holes", B, Lk)
+    spaced = torch.ones(B, 2 * Lk, dtype=torch.bool, device="cuda")
+    spaced[:, ::2] = hidden
+    for mask in (hidden.t().contiguous().t(), spaced[:, ::2], hidden[:1].expand(B, Lk), hidden[:, :1].expand(B, Lk)):
+        assert not mask.is_contiguous()
+        saved = T.attention_forward(q, k, v, mask, causal)
+        want = T.attention_forward(q, k, v, mask.contiguous(), causal)
+        assert torch.equal(saved[0], want[0]) and torch.equal(saved[1][0], want[1][0])
+        for a, b in zip(T.attention_backward(do, q, k, v, *saved, mask, causal), T.attention_backward(do, q, k, v, *want, mask.contiguous(), causal)):
+            assert torch.equal(a, b)
+    check_attention(q, k, v, do, spaced[:, ::2], causal, D ** -0.5, "spaced")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(2, 1, 700, 8, 2, 128), (2, 150, 150, 4, 2, 128), (1, 600, 600, 2, 2, 96), (32, 300, 40, 8, 8, 64)], ids=lambda s: "x".join(map(str, s)))
+def test_wide_heads_captured_and_replayed(shape, dtype):
+    """Kernels with more than 64 KB of LDS, which is asked for at their launch, and splits with their join, in a graph that is replayed on new data between eager work."""
+    B, Lq, Lk, H, Hk, D = shape
+    mask = key_mask("lengths", B, Lk)
+
+    def program(q, k, v, do):
+        out, saved = T.attention_forward(q, k, v, mask)
+        return (out, saved[0], *T.attention_backward(do, q, k, v, out, saved, mask))
+
+    def data(seed):
+        return [*heads("tokens", *shape, dtype, seed), rnd(B, Lq, H, D, seed=seed + 5, dtype=dtype)]
+
+    held, side, graph = data(50), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        program(*held)
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph):
+        got = program(*held)
+    for seed in (60, 70, 80):
+        fresh = data(seed)
+        for a, b in zip(held, fresh):
+            a.copy_(b)
+        graph.replay()
+        want = program(*fresh)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), seed
