@@ -53,7 +53,7 @@ def _first_order(what):
 
 
 def _int(what, *sizes):
-    if any(n >> 31 for n in sizes):
+    if max(sizes) >> 31:
         raise RuntimeError(f"tatt_amd {what}: a dimension of 2^31 or more, got {sizes}")      # the C ABI would get its low 32 bits
 
 
@@ -62,8 +62,8 @@ def _no_tangent(what, *tensors):
         raise NotImplementedError(f"tatt_amd {what}: no forward-mode derivatives")      # the result would have none, as if they were zero
 
 
-def _constant(what, *values):
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in values):
+def _constant(what, required):
+    if required and torch.is_grad_enabled():
         raise NotImplementedError(f"tatt_amd {what}: no gradient of a value that requires one")     # autograd would leave it None
 
 
@@ -166,7 +166,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
     """LayerNorm over the last dimension of x (float32 or bfloat16; weight and bias float32 or None), of any width below 2^27.  With a residual:
     -> (LayerNorm(sum), sum), sum = x + residual rounded to x's type, in one pass."""
     _no_tangent("layer_norm", x, residual, weight, bias, eps)
-    _constant("layer_norm: eps", eps)
+    _constant("layer_norm: eps", isinstance(eps, torch.Tensor) and eps.requires_grad)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight, bias)):
         return _LayerNormFn.apply(x, residual, weight, bias, eps)
     y, s, _ = layer_norm_forward(x, weight, bias, eps, residual, need_stat=False)
@@ -235,7 +235,7 @@ def rotary(q, k, positions, freqs, sections, interleaved=False):
     sections[1] by positions[..., 1] and so on, the rest passes through; freqs = rotary_frequencies(sections).  Positions and freqs have no
     gradient (refused if they require one).  -> (q', k'), or q' if k is None."""
     _no_tangent("rotary", q, k, positions, freqs)
-    _constant("rotary: positions and freqs", positions, freqs)
+    _constant("rotary: positions and freqs", positions.requires_grad or freqs.requires_grad)
     sections = tuple(int(s) for s in sections)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _RotaryFn.apply(q, k, positions, freqs, sections, bool(interleaved))
@@ -345,7 +345,7 @@ def attention(q, k, v, key_padding_mask=None, causal=False, scale=None):
     causality hides it included (0 times it).  float32 keeps its accuracy for magnitudes of 2^-100 to 2^127, scores (scaled) for magnitudes below
     2^28, past which a row may be NaN; the gradients' probabilities are off by 2^-24 of the score, relative to themselves."""
     _no_tangent("attention", q, k, v, scale)
-    _constant("attention: scale", scale)
+    _constant("attention: scale", isinstance(scale, torch.Tensor) and scale.requires_grad)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _AttentionFn.apply(q, k, v, key_padding_mask, causal, scale)
     return attention_forward(q, k, v, key_padding_mask, causal, scale, need_saved=False)[0]
