@@ -102,7 +102,9 @@ __device__ __forceinline__ Frag<T, COMPUTED<T>> pack_step(const f32x16& c, int s
 }
 
 // waves a SIMD that the registers are shared out for.  Two (256 registers each) unless what a wave has to hold -- the fragments of its rows, the
-// sums, a tile on its way -- would spill: then one (dK and dV of 128 in bf16: 384 us with two and 187 spilled registers, 230 with one).
+// sums, a tile on its way -- would spill: then one (dK and dV of 2 x 2777 tokens, 16 / 4 heads of 128, in bf16: 1129 us with two and 318 spilled registers,
+// 408 with one and none).  With one, fp32 dK and dV still spill: heads of 128 and few keys of 64 101 registers, of 96 53, into the accumulators' half of the
+// register file but for 58 of the 128's, which go to memory.
 template <typename T>
 constexpr int fwd_waves(int DK) { return sizeof(T) == 4 && DK > 64 ? 1 : 2; }
 template <typename T>
@@ -200,8 +202,8 @@ struct Where {
 };
 // Workgroups go round the 8 XCDs in turn, and to the CUs in order.
 // Causal: blocks differ in length, so the long ones of every problem go first (blocks: the slowest index, w.blk = 0 the longest), and the short ones
-// fill up what they leave (4 x 4096, 8 heads of 64, bf16: training 527 -> 437 us).  With a mask the problems differ too and are turned against the
-// XCDs, lest a short sequence leave an XCD idle (two clips, one of them empty: dQ 141 -> 128 us).
+// fill up what they leave (4 x 4096, 8 heads of 64, bf16: kernels of a training pass 683 -> 553 us).  With a mask the problems differ too and are turned against the
+// XCDs, lest a short sequence leave an XCD idle (two clips, one of them empty: dQ 146 -> 132 us).
 // Else each XCD gets a contiguous range of the work, so that the blocks that read one key head share an L2 (fp32, 16 x 4 heads of 1024: 2-6 %
 // faster) -- but not where the work of a range may differ, with a mask, or with splits, which share nothing.
 __device__ __forceinline__ Where where(const MhaArgs& a) {
@@ -228,7 +230,7 @@ __device__ __forceinline__ Where where(const MhaArgs& a) {
 }
 
 // One split of the summed axis' places [lo, hi): the split's length, or, where causality has cut that axis differently for every block, an equal share of
-// what is left of it in whole tiles (dK and dV of 2 x 2777, 4 key heads of 128: 177 -> 162 us).
+// what is left of it in whole tiles (dK and dV of 2 x 2777, 16 / 4 heads of 128: 308 -> 214 us).
 __device__ __forceinline__ void take_split(const MhaArgs& a, int split, int tile, int& lo, int& hi) {
   if (a.nsplit == 1) return;
   const int all = max(0, hi - lo), per = a.causal ? ((all + a.nsplit - 1) / a.nsplit + tile - 1) / tile * tile : a.per_split;
@@ -499,11 +501,12 @@ struct Plan {
   int wide, nblk, nsplit, per_split;  // wide: waves side by side along the output axis; else along the summed one
 };
 // Blocks of 128 along the output axis, 32 if it has no more than 32, and the summed axis in splits of no less than `finest`.
-// One tile of rows: as many splits as fill the chip twice (sequences differ in length).  `whole`, workgroups that work on 128: as few as make the pass
+// One tile of rows: where blocks do not fill the chip, as many splits as fill it twice (sequences differ in length), and none where they do: 63 sequences of
+// up to 20000 keys, 8 key heads of 128, bf16, take 623 + 5 us in three splits, 64 of them 773 in one.  `whole`, workgroups that work on 128: as few as make the pass
 // shortest, with `slots` workgroups at a time, in units of a whole block: the workgroups that a CU gets one after another (of two at a time, the last alone
 // takes 0.6), or, where causal, the longest of them and their even share; and the partial sums, written and read, `traffic` / inner of the products' time a
-// split.  (bf16, heads of 128, dK and dV: 8 x 1024 x 4 in 56 us unsplit and 80 + 16 in four splits, 2 x 2777 x 16 / 4 in 396 + 20 in four and 436 + 31 in
-// six.)
+// split.  (bf16, heads of 128, dK and dV: 8 x 1024 x 4 in 58 us unsplit and 84 + 23 in four splits, 2 x 2777 x 16 / 4 in 498 unsplit, 408 + 21 in four and 460
+// with the sum still to come in six.)
 inline Plan plan(long problems, int outer, int inner, int finest, int causal, int slots, float traffic, bool whole) {
   Plan p;
   p.wide = outer > 32;
@@ -529,7 +532,8 @@ inline Plan plan(long problems, int outer, int inner, int finest, int causal, in
   return p;
 }
 
-// workgroups of four waves that the chip holds at once, and plan()'s `traffic`: fp32 products take some five times as long
+// workgroups of four waves that the chip holds at once, and plan()'s `traffic`: fp32 products take some four times as long (the measured shapes are split
+// alike with 280 for bf16)
 inline int slots_of(int waves) { return waves == 1 ? 256 : 512; }
 inline float traffic_of(int dtype) { return dtype == TATT_T_BF16 ? 400.f : 80.f; }
 

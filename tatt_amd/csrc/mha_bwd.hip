@@ -2,10 +2,11 @@
 // The probabilities are recomputed from lse, once in the kernel whose rows are queries (dQ, and delta on the way) and once in the one whose rows
 // are keys (dK, dV): seven products instead of the five that atomics into dQ would need, and sums in a fixed order.
 //
-// Bound like the forward pass, with three products and four to an exponential.  Measured (executed products): 4 x 4096 tokens, 8 heads of 64,
-// bf16: dQ 233 us, 885 TFLOP/s (64 rows a wave; with 32: 248), dK and dV 304 us, 904 TFLOP/s (tiles of 128 rows; of 64: 351); 16 x 1024, 4 heads of 64,
-// fp32: 177 us (146) and 225 us (153); heads of 128 in bf16, 2 x 2777 tokens of 16 heads: 232 us (815) and 393 + 23 for the sum over four splits
-// (640: a wave has its SIMD for itself, nothing fills its waits), for one causal clip of them 126 and 168 + 17.
+// Bound like the forward pass: to an exponential, dQ has three products and dK and dV four, those of P and dS by two pieces where tensors are bf16 (four and
+// six executed).  Measured, at the clock that a busy chip keeps (executed products): 4 x 4096 tokens, 8 heads of 64, bf16: dQ 264 us, 1040 TFLOP/s (64 rows a
+// wave; with 32: 289), dK and dV 391 us, 1055 TFLOP/s (tiles of 128 rows; of 64: 402); 16 x 1024, 4 heads of 64, fp32: 151 us (171, fp32 products) and 192 us
+// (179); heads of 128 in bf16, 4 x 2816 tokens of 16 heads: 498 us (1043) and 825 (945); 2 x 2777 of 16 / 4: 268 (942) and 408 + 21 for the sum over four
+// splits (929), for one causal clip of them 88 + 16 and 117 + 16.
 #include "mha.h"
 
 namespace {
@@ -318,7 +319,7 @@ __global__ __launch_bounds__(256) void mha_sum_kernel(const float* __restrict__ 
   (i < n ? y : y2)[i < n ? i : i - n] = from_f32<T>(s);
 }
 
-// Splits of no less than 256 (2 x 1024 x 1024, 4 heads of 64: fp32 70 us against 104 with 512, bf16 39 against 44; with 128 94 and 51)
+// Splits of no less than 256 (2 x 1024 x 1024, 4 heads of 64: kernels fp32 69 us against 103 with 512, bf16 41 against 51; with 128 the same)
 Plan plan_dq(int B, int Lq, int Lk, int H, int Hkv, int D, int causal, int dtype) {
   return plan((long)B * Hkv, Lq * (H / Hkv), Lk, 256, causal, slots_of(dtype == TATT_T_BF16 ? dq_waves<bf16_t>(D) : dq_waves<float>(D > 32 ? 64 : D)), traffic_of(dtype), true);
 }
@@ -361,7 +362,7 @@ int run_bwd(MhaArgs& a, T* dq, T* dk, T* dv, float* part, hipStream_t st) {
     }
   if (rc < 0) {
     a.nblk = cdiv(a.rows, 128);
-    // tiles of 64 keys (heads of 128: 132 us against 148 with 32), of 32 where three pieces of them would not fit
+    // tiles of 64 keys (2 x 2777, 16 / 4 heads of 128: 268 us against 277 with 32), of 32 where three pieces of them would not fit
     rc = launch_dq<T, DK, 1, (DK > 64 && sizeof(T) == 4 ? 1 : 2)>(a, dq, q_part, st);
   }
   if (rc) return rc;
@@ -378,7 +379,7 @@ int run_bwd(MhaArgs& a, T* dq, T* dk, T* dv, float* part, hipStream_t st) {
   // buffer 45)
   if constexpr (sizeof(T) == 4 && DK > 64)
     rc = launch_dkv<T, DK, 4, 1, 1>(a, dk, dv, kv_part, st);
-  else if (p.wide)  // row tiles of 128 for narrow bf16 heads, 64 for wide ones (178 us against 226 with 32), 32 in fp32: what two buffers leave room for
+  else if (p.wide)  // row tiles of 128 for narrow bf16 heads, 64 for wide ones (2 x 2777, 16 / 4 of 128: 408 us against 498 with 32), 32 in fp32: what two buffers leave room for
     rc = launch_dkv<T, DK, 4, 1, (sizeof(T) == 4 ? 1 : DK > 64 ? 2 : 4)>(a, dk, dv, kv_part, st);
   else
     rc = launch_dkv<T, DK, 1, (sizeof(T) == 4 ? 4 : narrow_waves<T>(DK)), 1>(a, dk, dv, kv_part, st);

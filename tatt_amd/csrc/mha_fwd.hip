@@ -1,14 +1,15 @@
 // Attention of any lengths, head counts and head widths up to 128, forward (attn.hip is the 26-key, 4 x 16 form; mha.h has the mathematics
 // and the layouts).  One pass over the keys with a running maximum and sum; no score leaves the registers.
 //
-// Bound: of a tile of 32 x 32 scores a wave issues D / 8 products of 32 cycles and some 110 vector instructions (maximum, exponential, sum, packing), and the
-// two hardly overlap within a wave; two waves a SIMD share it.  Keys come through LDS, 64 a tile, two buffers, loaded a tile ahead.
+// Bound: of a tile of 32 x 32 scores a wave issues D / 16 products of 32 cycles for the scores, D / 8 (P in two pieces, bf16) for the output and some
+// 150 vector instructions (maximum, exponential, sum, packing), and the two hardly overlap within a wave; two waves a SIMD share it.  Keys come
+// through LDS, 64 a tile, two buffers, loaded a tile ahead.
 // 64 rows a wave (R = 2) read every fragment from LDS once for two products; 32 keep more workgroups where rows are few, and the registers of
-// heads wider than 64 hold no more.  Measured: 4 x 4096 tokens, 8 heads of 64, bf16: 189 us, 727 TFLOP/s (R = 1: 254 us); 16 x 1024, 4 heads of
-// 64, fp32: 99 us, 174 TFLOP/s; 2816 keys, 128 queries to a workgroup, heads of 128, bf16: 880 TFLOP/s with the chip full, 325 for one causal clip
-// of 2777 tokens, whose longest blocks take 44 tiles while others have ended.
-// A single query reads its keys at 3.4 TB/s (8 x 20000 keys, 8 key heads of 128, bf16: 97 us): the keys are split over workgroups, one tile of rows each
-// (the G heads of a key head), with the sums joined afterwards.
+// heads wider than 64 hold no more.  Measured, at the clock that a busy chip keeps: 4 x 4096 tokens, 8 heads of 64, bf16: 228 us,
+// 904 TFLOP/s of executed products (R = 1: 249 us); 16 x 1024, 4 heads of 64, fp32: 92 us, 186 TFLOP/s of fp32 products; 4 x 2816, 16 heads of 128, bf16:
+// 401 us, 972 TFLOP/s; one causal clip of 2777 tokens, 16 / 4 heads of 128, in three splits: 62 us, 770 TFLOP/s, and 18 to 22 for the join.
+// A single query reads its keys at 3.1 TB/s, half of what reading alone reaches (8 sequences of up to 20000 keys, 8 key heads of 128, bf16: 107 us): the keys
+// are split over workgroups, one tile of rows each (the G heads of a key head), with the sums joined afterwards.
 #include "mha.h"
 
 namespace {
@@ -80,7 +81,8 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
     __syncthreads();
   }
   // One version of the loop's body, conditions around single steps only: the accumulators stay where they are (with a version for whole tiles
-  // beside one for masked ones the compiler copied them every tile, waiting for the products to do so: 226 us against 190, 4 x 4096, 8 x 64, bf16).
+  // beside one for masked ones the compiler copied them every tile, waiting for the products to do so: 226 us against 190, 4 x 4096, 8 x 64, bf16, P in
+  // one piece).
   for (int k0 = kbeg; k0 < kend; k0 += KT) {
     if (NB == 1 && k0 + KT < kend) fetch(k0 + KT);
     const char *kt = lds + at, *vt = kt + TILE;
@@ -231,8 +233,8 @@ __global__ __launch_bounds__(64 * WQ * WK, fwd_waves<T>(DK)) void mha_fwd_kernel
 }
 
 // The splits of a row, a wave per row.  Lane = split for the weights; then D / 4 lanes (LPR, rounded up to a power of two) hold four dimensions
-// each, and as many groups of them as the wave has take the splits in turn.  Bound by memory: 256 rows of 39 splits 4.5 us, 44432 rows of two splits
-// (57 MB) 23 us.
+// each, and as many groups of them as the wave has take the splits in turn.  Bound by memory: 256 rows of 16 splits 5 us, 44432 rows of three splits
+// (80 MB) 18 to 22 us.
 template <typename T, int LPR>
 __global__ __launch_bounds__(256) void mha_fwd_join(const float* __restrict__ part, int nsplit, long R, int D, int H, int Lq, T* __restrict__ out, bf16_t* __restrict__ low,
                                                     float* __restrict__ lse) {
@@ -284,10 +286,10 @@ __global__ __launch_bounds__(256) void mha_fwd_join(const float* __restrict__ pa
 }
 
 // A split costs its partial sums, a second launch and the workspace: with bf16 tiles, done quickly, 512 keys are worth that (8 x 8 heads of 64, one query,
-// 1000 keys: 12 us unsplit and 16 in splits of 256; 20000 keys, 32 / 8 heads of 128: 149 in splits and 447 without), with fp32 ones 128 (17 us in splits
+// 1000 keys: 14.6 us unsplit, 9.3 and 3.3 with a launch between in splits of 256), with fp32 ones 128 (17 us in splits
 // of 128 and 28 of 512; one query, 4000 keys, 8 key heads of 128: 43 and 92; with two waves, below, 29).
-// Workgroups at once: of one wave and 48 KB (fp32 heads past 64, few rows) three a CU (8 x 20000 keys, 8 heads of 128, one query: 317 us in 23 splits,
-// 402 in 8).
+// Workgroups at once: of one wave and 48 KB (fp32 heads past 64, few rows) three a CU (8 sequences of up to 20000 keys, 8 heads of 128, one query: 244 us in
+// 23 splits, 424 in the 16 of two a CU; all of them of 20000: 292).
 Plan plan_fwd(int B, int Lq, int Lk, int H, int Hkv, int D, int causal, int dtype) {
   const bool bf16 = dtype == TATT_T_BF16;
   const int rows = Lq * (H / Hkv), slots = rows > 32 ? slots_of(bf16 ? fwd_waves<bf16_t>(D) : fwd_waves<float>(D)) : !bf16 && D > 64 ? 768 : 512;
@@ -320,7 +322,7 @@ int run_fwd(MhaArgs& a, T* out, bf16_t* low, float* lse, float* part, hipStream_
     // where they do not, more waves do (8 x 32 heads of 128, one query: 300 keys 43 us with 1 wave and 30 with 2, 20000 keys 385 and 440)
     const bool filled = (long)a.B * a.Hkv * p.nblk * p.nsplit >= 512;
     rc = filled ? launch_fwd<T, DK, 1, 1, WK, 1, 1>(a, out, low, lse, part, st) : launch_fwd<T, DK, 1, 1, MORE, 1, 1>(a, out, low, lse, part, st);
-  } else if constexpr (sizeof(T) == 2 && DK <= 64) {  // 64 rows a wave where that leaves a workgroup to every CU (190 us against 254, above)
+  } else if constexpr (sizeof(T) == 2 && DK <= 64) {  // 64 rows a wave where that leaves a workgroup to every CU (228 us against 249, above)
     if ((long)a.B * a.Hkv * a.nsplit * cdiv(a.rows, 256) >= 256) {
       a.nblk = cdiv(a.rows, 256);
       rc = launch_fwd<T, DK, 4, 2, 1, 2, 2>(a, out, low, lse, part, st);

@@ -339,7 +339,7 @@ def attention(q, k, v, key_padding_mask=None, causal=False, scale=None):
     """softmax(scale q k^T) v per head, the scores never in memory.  q [B, Lq, H, D], k and v [B, Lk, Hk, D] (float32 or bfloat16, any
     strides, D <= 128), H a multiple of Hk: query head h reads key head h // (H // Hk).  key_padding_mask [B, Lk] bool, True = leave the key out (as
     nn.MultiheadAttention's): nothing of such a key reaches a result.  causal: query i sees keys j <= i + Lk - Lq.  scale: D ** -0.5 if None.  A row
-    that sees no key gives zeros and takes no part in any gradient.  -> out [B, Lq, H, D].
+    that sees no key gives zeros and takes no part in any gradient.  No dropout.  -> out [B, Lq, H, D].
 
     What is not masked is expected to be finite: an infinity or NaN spreads to what a matrix product with it would reach, the rows from which only
     causality hides it included (0 times it).  float32 keeps its accuracy for magnitudes of 2^-100 to 2^127, scores (scaled) for magnitudes below
