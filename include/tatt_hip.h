@@ -393,7 +393,8 @@ int tatt_rotary(const void* q, const long* q_strides, void* q_out, int Hq, const
  * exponentials, and, for bf16 tensors, out_low like out = what rounding took from out, which the backward call adds again in its row sums dO . O (both NULL
  * if no backward call follows; out_low may be).  A row that sees no key gives zeros, lse = +inf, and no gradient;
  * scores past 2^29 give NaN.  The backward call recomputes the probabilities from lse; dq, dk, dv contiguous.
- * workspace: tatt_mha_*_workspace floats, 16-byte aligned (0 = may be NULL). */
+ * Fewer than 2^30 rows (B H Lq, B Hkv Lk), at most 65536 query heads to a key head.  workspace: tatt_mha_*_workspace floats, 16-byte aligned (0 = may be
+ * NULL; also 0 for sizes that are refused). */
 size_t tatt_mha_fwd_workspace(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype);
 int tatt_mha_fwd(const void* q, const void* k, const void* v, const long* strides, const unsigned char* key_mask, const long* mask_strides, void* out, void* out_low, float* lse, int B, int Lq, int Lk, int H, int Hkv, int D, float scale, int causal, int dtype, float* workspace, hipStream_t stream);
 size_t tatt_mha_bwd_workspace(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype);
